@@ -9,7 +9,7 @@ from . import build
 _u8p, _f32p, _i32p, _u32p, _u16p = (C.POINTER(t) for t in (C.c_uint8, C.c_float, C.c_int32, C.c_uint32, C.c_uint16))
 _vp, _sz, _cp = C.c_void_p, C.c_size_t, C.c_char_p
 
-# name -> (restype, argtypes); every symbol include/m26s_b1.h, include/m26c_glue.h and include/m26w_frame.h declare
+# name -> (restype, argtypes); every symbol include/m26s_b1.h, m26c_glue.h, m26c_coord.h and m26w_frame.h declare
 SIGNATURES = {
     "m26w_crc32c_update": (C.c_uint32, [C.c_uint32, _vp, _sz]),
     "m26w_crc32c_update_portable": (C.c_uint32, [C.c_uint32, _vp, _sz]),
@@ -23,6 +23,14 @@ SIGNATURES = {
     "m26c_rank_sum_bf16": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_long, _vp]),
     "m26c_add_inplace": (C.c_int, [_vp, _vp, C.c_long, _vp]),
     "m26c_f32_to_bf16": (C.c_int, [_vp, _vp, C.c_long, _vp]),
+    "m26c_block_join": (C.c_int, [_vp, C.c_long, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "m26c_w4_new": (C.c_int, [_vp, _vp, C.c_long, C.c_long, _vp, C.POINTER(_vp), _cp, _sz]),
+    "m26c_w4_free": (None, [_vp]),
+    "m26c_w4_matvec": (C.c_int, [_vp, _vp, C.c_long, C.c_int, _vp, C.c_int, C.c_long, _vp]),
+    "m26c_w4_matvec_fp8": (C.c_int, [_vp, _vp, _sz, _vp, _sz, C.c_int, _vp, C.c_int, C.c_long, _vp]),
+    "m26c_token_logprobs_workspace": (_sz, [C.c_int, C.c_int, C.c_int]),
+    "m26c_token_logprobs": (C.c_int, [_vp, C.c_int, C.c_long, C.c_int, C.c_int, C.c_float, _vp, C.c_int, _vp, _vp, C.c_int, _vp, _vp, _vp,
+                                      _sz, _vp]),
     "m26s_b1_layer_new": (C.c_int, [_vp, C.c_uint64, C.c_uint32, C.POINTER(_vp), _cp, _sz]),
     "m26s_b1_layer_all_normal": (C.c_int, [_vp]),
     "m26s_b1_layer_free": (None, [_vp]),

@@ -1,6 +1,6 @@
 """Builds the HIP libraries (gfx950) in-tree with hipcc. No GPU is needed to compile.
 
-lib/libm26s_b1.so   the serving library: the expert FFN, the coordinator-side kernels, the frame adapter
+lib/libm26s_b1.so   the serving library: the expert FFN, the coordinator-side kernels and operators, the frame adapter
 lib/libm26_probe.so measurement aids only (what the GPU sustains on the two rooflines); the serving
                     library does not carry them, and only the benchmark and one test load them
 """
@@ -13,9 +13,10 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "lib", "libm26s_b1.so")
 PROBE_LIB = os.path.join(HERE, "lib", "libm26_probe.so")
-SOURCES = ["csrc/b1_abi.hip", "csrc/glue_abi.hip", "csrc/frame_abi.hip"]
+SOURCES = ["csrc/b1_abi.hip", "csrc/glue_abi.hip", "csrc/coord_abi.hip", "csrc/frame_abi.hip"]
 DEPENDS = ["csrc/b1_kernels.h", "csrc/b1_tile.h", "csrc/b1_conform.h", "csrc/b1_layout.h", "csrc/glue_kernels.h",
-           "../include/m26s_b1.h", "../include/m26c_glue.h", "../include/m26w_frame.h"]
+           "csrc/q0_codec.h", "csrc/join_kernels.h", "csrc/w4_kernels.h", "csrc/logprob_kernels.h",
+           "../include/m26s_b1.h", "../include/m26c_glue.h", "../include/m26c_coord.h", "../include/m26w_frame.h"]
 PROBE_SOURCES = ["csrc/probe_abi.hip"]
 PROBE_DEPENDS = ["../include/m26_probe.h"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off",

@@ -1,0 +1,256 @@
+// C ABI of the coordinator-side operators (include/m26c_coord.h): argument checks and launches.
+#include "../../include/m26c_coord.h"
+#include <cmath>
+#include <new>
+#include <stdio.h>
+#include "join_kernels.h"
+#include "logprob_kernels.h"
+#include "w4_kernels.h"
+
+namespace {
+
+using namespace m26g;
+
+int launched() { return int(hipGetLastError()); }
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+bool on(const void* p, uintptr_t boundary) { return address(p) % boundary == 0; }
+
+// ---- block join
+template <int T, int NG>
+void launch_join(const JoinArgs& a, bool vec, unsigned grid, hipStream_t st) {
+    if (vec) block_join_kernel<T, NG, true><<<grid, T, 0, st>>>(a);
+    else block_join_kernel<T, NG, false><<<grid, T, 0, st>>>(a);
+}
+
+// ---- log probabilities
+// Segments of a row: enough workgroups for four per compute unit where the rows alone are too few, but at least
+// two chunks for each of a workgroup's waves.
+int segments_of(int rows, int vocab) {
+    const long chunks = (long(vocab) + kChunk - 1) / kChunk;
+    long s = (1024 + rows - 1) / rows;
+    const long most = chunks / (2 * kLogprobWaves);
+    s = s < most ? s : most;
+    s = s < kSegmentsMost ? s : kSegmentsMost;
+    return int(s < 1 ? 1 : s);
+}
+size_t stats_bytes(int rows, int segments) { return size_t(rows) * segments * sizeof(float4); }
+
+template <bool BF16>
+int launch_logprobs(LogprobArgs a, hipStream_t st) {
+    if (a.segments == 1) {
+        const size_t size = BF16 ? 2 : 4;
+        for (int done = 0; done < a.rows;) {  // a launch holds under 2^32 threads
+            const int n = a.rows - done < (1 << 23) ? a.rows - done : (1 << 23);
+            LogprobArgs b = a;
+            b.rows = n;
+            b.logits = static_cast<const char*>(a.logits) + size_t(done) * a.pitch * size;
+            if (a.n_given) { b.given = a.given + size_t(done) * a.n_given; b.given_logprob = a.given_logprob + size_t(done) * a.n_given; }
+            if (a.entropy) b.entropy = a.entropy + done;
+            if (a.top) { b.top_ids = a.top_ids + size_t(done) * a.top; b.top_logprob = a.top_logprob + size_t(done) * a.top; }
+            logprob_kernel<BF16><<<unsigned(n), 64 * kLogprobWaves, 0, st>>>(b);
+            if (int rc = launched()) return rc;
+            done += n;
+        }
+        return 0;
+    }
+    logprob_kernel<BF16><<<unsigned(a.rows) * unsigned(a.segments), 64 * kLogprobWaves, 0, st>>>(a);
+    if (int rc = launched()) return rc;
+    logprob_join_kernel<BF16><<<unsigned(a.rows), 256, size_t(a.segments) * a.top * 8, st>>>(a);
+    return launched();
+}
+
+}  // namespace
+
+// ---- MXFP4 weights
+struct m26c_w4 {
+    W4Layout lay;
+    uint8_t* payload;
+    uint32_t* scales;
+    int device;
+};
+
+namespace {
+
+int fail(char* err, size_t errlen, int rc, const char* what) {
+    if (err && errlen) snprintf(err, errlen, "%s", what);
+    return rc;
+}
+
+void release(m26c_w4* w) {
+    if (!w) return;
+    if (w->payload) (void)hipFree(w->payload);
+    if (w->scales) (void)hipFree(w->scales);
+    delete w;
+}
+
+template <int TT>
+int launch_w4(const W4Args& args, bool fp8, hipStream_t st) {
+    constexpr long kMost = 65535L * 16 * TT;  // rows of one launch
+    for (long done = 0; done < args.rows; done += kMost) {
+        W4Args a = args;
+        const long n = args.rows - done < kMost ? args.rows - done : kMost;
+        a.rows = int(n);
+        if (fp8) {
+            a.x_codes += done * a.x_pitch;
+            a.x_scales += done * a.x_scales_pitch;
+        } else {
+            a.x += done * a.x_pitch;
+        }
+        a.y = static_cast<char*>(a.y) + done * a.y_pitch * (a.y_bf16 ? 2 : 4);
+        const dim3 grid(unsigned(a.w.tiles), unsigned((n + 16 * TT - 1) / (16 * TT)));
+        if (fp8) w4_matvec_kernel<TT, true><<<grid, 512, 0, st>>>(a);
+        else w4_matvec_kernel<TT, false><<<grid, 512, 0, st>>>(a);
+        if (int rc = launched()) return rc;
+    }
+    return 0;
+}
+
+int w4_run(const m26c_w4* w, W4Args a, bool fp8, void* stream) {
+    if (!w || a.rows < 0) return 1;
+    if (a.rows == 0) return 0;
+    int device = -1;
+    if (hipGetDevice(&device) != hipSuccess || device != w->device) return 1;
+    if (!a.y || a.y_pitch < w->lay.n || !on(a.y, a.y_bf16 ? 2 : 4)) return 1;
+    a.w = w->lay;
+    a.payload = w->payload;
+    a.scales = w->scales;
+    hipStream_t st = hipStream_t(stream);
+    if (a.rows <= 16) return launch_w4<1>(a, fp8, st);
+    if (a.rows <= 32) return launch_w4<2>(a, fp8, st);
+    return launch_w4<4>(a, fp8, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int m26c_block_join(const m26c_join* plan, long rows, const float* h, const uint16_t* p0, const uint16_t* p1, const uint16_t* p2,
+                    const uint16_t* p3, const float* gate, float* h_out, uint16_t* norm, uint8_t* payload, uint8_t* scales,
+                    void* stream) {
+    if (!plan || rows < 0) return 1;
+    const m26c_join& p = *plan;
+    const uint16_t* planes[4] = {p0, p1, p2, p3};
+    if (p.cols <= 0 || p.cols > 16384 || p.planes < 1 || p.planes > 4 || p.plane_pitch < p.cols || p.h_pitch < p.cols ||
+        !(p.eps > 0.0f) || !std::isfinite(p.eps) || !std::isfinite(p.scale) || (p.gate_cols != 0 && p.gate_cols != 1 && p.gate_cols != p.cols) ||
+        (p.gate_cols && (p.gate_pitch < 0 || (p.gate_pitch && p.gate_pitch < p.gate_cols))))
+        return 1;
+    if (rows == 0) return 0;
+    const bool normed = norm || payload;
+    if (!h || (!h_out && !normed) || (normed && !p.pre_weight) || (p.gate_cols && !gate) || !payload != !scales ||
+        (norm && p.norm_pitch < p.cols))
+        return 1;
+    if (payload && (p.cols % 32 || p.payload_pitch < size_t(p.cols) || p.scales_pitch < size_t(p.cols / 32))) return 1;
+    bool vec = p.cols % 8 == 0 && p.plane_pitch % 8 == 0 && p.h_pitch % 4 == 0 && on(h, 16) && on(h_out, 16) && on(norm, 16) &&
+               (!norm || p.norm_pitch % 8 == 0) && on(p.pre_weight, 16) && on(p.post_weight, 16) && on(payload, 8) &&
+               (!payload || p.payload_pitch % 8 == 0);
+    if (!on(h, 4) || !on(h_out, 4) || !on(norm, 2) || !on(p.pre_weight, 4) || !on(p.post_weight, 4)) return 1;
+    for (int i = 0; i < p.planes; ++i) {
+        if (!planes[i] || !on(planes[i], 2)) return 1;
+        vec = vec && on(planes[i], 16);
+    }
+    if (p.gate_cols) {
+        if (!on(gate, 4)) return 1;
+        if (p.gate_cols > 1) vec = vec && on(gate, 16) && p.gate_pitch % 4 == 0;
+    }
+    JoinArgs a{};
+    for (int i = 0; i < p.planes; ++i) a.plane[i] = planes[i];
+    a.h = h; a.gate = gate; a.pre_w = p.pre_weight; a.post_w = p.post_weight;
+    a.h_out = h_out; a.norm = norm; a.payload = payload; a.scales = scales;
+    a.rows = rows; a.plane_pitch = p.plane_pitch; a.h_pitch = p.h_pitch; a.norm_pitch = p.norm_pitch; a.gate_pitch = p.gate_pitch;
+    a.payload_pitch = p.payload_pitch; a.scales_pitch = p.scales_pitch;
+    a.cols = p.cols; a.planes = p.planes; a.gate_cols = p.gate_cols; a.scale = p.scale; a.eps = p.eps;
+    const unsigned grid = unsigned(rows < 65536 ? rows : 65536);
+    hipStream_t st = hipStream_t(stream);
+    if (p.cols <= 2048) launch_join<256, 1>(a, vec, grid, st);
+    else if (p.cols <= 4096) launch_join<256, 2>(a, vec, grid, st);
+    else if (p.cols <= 8192) launch_join<512, 2>(a, vec, grid, st);
+    else launch_join<1024, 2>(a, vec, grid, st);
+    return launched();
+}
+
+int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, void* stream, m26c_w4** out, char* err, size_t errlen) {
+    if (!out) return fail(err, errlen, 1, "w4 weights: no place for the handle");
+    *out = nullptr;
+    if (!payload || !scales || n <= 0 || k <= 0 || k % 32 || n > (1L << 26) || k > (1L << 24)) return fail(err, errlen, 1, "w4 weights: bad pointers or sizes");
+    if (!on(payload, 16)) return fail(err, errlen, 1, "w4 weights: the payload has to be 16-byte aligned");
+    m26c_w4* w = new (std::nothrow) m26c_w4{};
+    if (!w) return fail(err, errlen, 2, "w4 weights: out of host memory");
+    w->lay = W4Layout{n, k, int((n + 15) / 16), int((k + 127) / 128), int((k + 511) / 512)};
+    const size_t payload_bytes = size_t(w->lay.tiles) * w->lay.steps * 1024, scale_bytes = size_t(w->lay.tiles) * w->lay.quads * 256;
+    uint32_t* fault = nullptr;
+    if (hipGetDevice(&w->device) != hipSuccess || hipMalloc(&w->payload, payload_bytes) != hipSuccess ||
+        hipMalloc(&w->scales, scale_bytes + 256) != hipSuccess) {
+        (void)hipGetLastError();
+        release(w);
+        return fail(err, errlen, 2, "w4 weights: device allocation failed");
+    }
+    fault = w->scales + scale_bytes / 4;  // one word behind the scales
+    hipStream_t st = hipStream_t(stream);
+    uint32_t seen = 0;
+    const long cells = long(w->lay.tiles) * w->lay.quads * 256;
+    const long blocks = (cells + 255) / 256;
+    hipError_t e = hipMemcpyAsync(fault, &seen, 4, hipMemcpyHostToDevice, st);
+    if (e == hipSuccess) {
+        w4_prepare_kernel<<<unsigned(blocks < 65536 ? blocks : 65536), 256, 0, st>>>(payload, scales, w->lay, w->payload, reinterpret_cast<uint8_t*>(w->scales), fault);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess) e = hipMemcpyAsync(&seen, fault, 4, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    if (e != hipSuccess || seen) {
+        release(w);
+        return e != hipSuccess ? fail(err, errlen, 2, hipGetErrorString(e))
+                               : fail(err, errlen, 3, "w4 weights: a scale byte outside 2..252 over a nonzero code");
+    }
+    *out = w;
+    return 0;
+}
+
+void m26c_w4_free(m26c_w4* w) { release(w); }
+
+int m26c_w4_matvec(const m26c_w4* w, const uint16_t* x, long x_pitch, int rows, void* y, int y_bf16, long y_pitch, void* stream) {
+    if (rows > 0 && (!w || !x || !on(x, 16) || x_pitch < w->lay.k || x_pitch % 8)) return 1;
+    W4Args a{};
+    a.x = x; a.x_pitch = x_pitch; a.rows = rows; a.y = y; a.y_bf16 = y_bf16 != 0; a.y_pitch = y_pitch;
+    return w4_run(w, a, false, stream);
+}
+
+int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_pitch, const uint8_t* scales, size_t scales_pitch,
+                       int rows, void* y, int y_bf16, long y_pitch, void* stream) {
+    if (rows > 0 && (!w || !payload || !scales || !on(payload, 8) || payload_pitch % 8 || payload_pitch < size_t(w->lay.k) ||
+                     scales_pitch < size_t(w->lay.k / 32) || payload_pitch > size_t(1) << 40 || scales_pitch > size_t(1) << 40))
+        return 1;
+    W4Args a{};
+    a.x_codes = payload; a.x_scales = scales; a.x_pitch = long(payload_pitch); a.x_scales_pitch = long(scales_pitch);
+    a.rows = rows; a.y = y; a.y_bf16 = y_bf16 != 0; a.y_pitch = y_pitch;
+    return w4_run(w, a, true, stream);
+}
+
+size_t m26c_token_logprobs_workspace(int rows, int vocab, int top) {
+    if (rows <= 0 || vocab <= 0 || top < 0 || top > kTopMost) return 0;
+    const int segments = segments_of(rows, vocab);
+    return segments == 1 ? 0 : stats_bytes(rows, segments) + size_t(rows) * segments * top * 8;
+}
+
+int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int vocab, float scale, const int* given, int n_given,
+                        float* given_logprob, float* entropy, int top, int* top_ids, float* top_logprob, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+    if (rows < 0 || vocab <= 0 || n_given < 0 || top < 0 || top > kTopMost || top > vocab || !(scale > 0.0f) || !std::isfinite(scale) || pitch < vocab) return 1;
+    if (rows == 0) return 0;
+    if (!logits || !on(logits, bf16 ? 2 : 4) || (n_given && (!given || !given_logprob || !on(given, 4) || !on(given_logprob, 4))) || !on(entropy, 4) ||
+        (top && (!top_ids || !top_logprob || !on(top_ids, 4) || !on(top_logprob, 4))))
+        return 1;
+    LogprobArgs a{};
+    a.segments = segments_of(rows, vocab);
+    const size_t need = m26c_token_logprobs_workspace(rows, vocab, top);
+    if (need && (!workspace || !on(workspace, 16) || workspace_bytes < need)) return 1;
+    a.logits = logits; a.pitch = pitch; a.rows = rows; a.vocab = vocab; a.scale = scale;
+    a.given = given; a.n_given = n_given; a.given_logprob = given_logprob; a.entropy = entropy;
+    a.top = top; a.top_ids = top_ids; a.top_logprob = top_logprob;
+    if (need) {
+        a.stats = static_cast<float4*>(workspace);
+        a.lists = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + stats_bytes(rows, a.segments));
+    }
+    return bf16 ? launch_logprobs<true>(a, hipStream_t(stream)) : launch_logprobs<false>(a, hipStream_t(stream));
+}
+
+}  // extern "C"
