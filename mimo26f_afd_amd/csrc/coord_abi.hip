@@ -83,6 +83,30 @@ void release(m26c_w4* w) {
     delete w;
 }
 
+// Rows that stay in registers: up to 32 rows, k up to 8192 (4096 for more than 16 rows). False if they do not fit.
+template <int TT, int S, int DEPTH>
+int launch_resident(const W4Args& a, bool fp8, hipStream_t st) {
+    const int slices = (a.w.steps + S - 1) / S, groups = 8 / slices, tiles = (a.w.tiles + groups - 1) / groups;
+    constexpr int kWorkgroups = 256;
+    const int turns = (tiles + kWorkgroups - 1) / kWorkgroups, wide = (tiles + turns - 1) / turns;
+    const dim3 grid(unsigned(wide), 1), block(unsigned(64 * slices * groups));
+    if (fp8) w4_resident_kernel<TT, S, DEPTH, true><<<grid, block, 0, st>>>(a, slices, groups, turns);
+    else w4_resident_kernel<TT, S, DEPTH, false><<<grid, block, 0, st>>>(a, slices, groups, turns);
+    return launched();
+}
+template <int TT>
+bool resident(const W4Args& a, bool fp8, hipStream_t st, int& rc) {
+    const int steps = a.w.steps;
+    if (steps <= 8) rc = launch_resident<TT, 1, 4>(a, fp8, st);
+    else if (steps <= 16) rc = launch_resident<TT, 2, 4>(a, fp8, st);
+    else if (steps <= 24) rc = launch_resident<TT, 3, 3>(a, fp8, st);
+    else if (steps <= 32) rc = launch_resident<TT, 4, 3>(a, fp8, st);
+    else if (TT == 1 && steps <= 48) rc = launch_resident<1, 6, 2>(a, fp8, st);
+    else if (TT == 1 && steps <= 64) rc = launch_resident<1, 8, 2>(a, fp8, st);
+    else return false;
+    return true;
+}
+
 template <int TT>
 int launch_w4(const W4Args& args, bool fp8, hipStream_t st) {
     constexpr long kMost = 65535L * 16 * TT;  // rows of one launch
@@ -115,6 +139,9 @@ int w4_run(const m26c_w4* w, W4Args a, bool fp8, void* stream) {
     a.payload = w->payload;
     a.scales = w->scales;
     hipStream_t st = hipStream_t(stream);
+    int rc = 0;
+    if (a.rows <= 16 && resident<1>(a, fp8, st, rc)) return rc;
+    if (a.rows > 16 && a.rows <= 32 && resident<2>(a, fp8, st, rc)) return rc;
     if (a.rows <= 16) return launch_w4<1>(a, fp8, st);
     if (a.rows <= 32) return launch_w4<2>(a, fp8, st);
     return launch_w4<4>(a, fp8, st);

@@ -117,6 +117,95 @@ __device__ __forceinline__ W4Group w4_load_x(const W4Args& a, long row, long gro
     return g;
 }
 
+typedef uint32_t v4u32 __attribute__((ext_vector_type(4)));
+
+// A run of memory with its end: loads past it return zero and move nothing, so a wave may ask for steps or tiles that are
+// not there without a branch (a load under a condition makes the compiler wait for everything in flight).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_run_of(const void* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
+}
+constexpr int kStreamed = 2;  // non-temporal: a weight is used once
+
+// Rows resident: x stays in registers. A workgroup's waves are `groups` column groups of `slices` k-slices, S steps each;
+// a wave converts its slice of 16 * TT rows to matrix operands once and then walks over tiles, DEPTH of them in flight, with
+// nothing but weights left to load. The slices' sums meet in LDS, in order, two buffers taking turns so that one
+// barrier per tile does.
+template <int TT, int S, int DEPTH, bool FP8>
+__global__ void __launch_bounds__(512) w4_resident_kernel(const W4Args a, int slices, int groups, int turns) {
+    __shared__ float sums[2][8][TT][256];
+    const int lane = threadIdx.x & 63, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave % slices, group = wave / slices;
+    const int row0 = blockIdx.y * 16 * TT, k_groups = int(a.w.k / 32);
+    const long tile0 = long(blockIdx.x) * groups + group, tile_stride = long(gridDim.x) * groups;
+    const uint32_t step_bytes = uint32_t(a.w.steps) * 1024, scale_bytes = uint32_t(a.w.quads) * 256;
+    struct Tile {
+        v4u32 codes[S];
+        uint32_t scales[S];
+    };
+    auto load = [&](long tile, Tile& t) {
+        const bool there = tile < a.w.tiles;
+        const long at = there ? tile : 0;
+        const __amdgpu_buffer_rsrc_t codes = w4_run_of(a.payload + at * step_bytes, there ? step_bytes : 0);
+        const __amdgpu_buffer_rsrc_t scales = w4_run_of(reinterpret_cast<const uint8_t*>(a.scales) + at * scale_bytes, there ? scale_bytes : 0);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int step = slice * S + s;
+            t.codes[s] = __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, step * 1024, kStreamed);
+            // one byte per step and lane; four neighbouring steps share a dword
+            t.scales[s] = __builtin_amdgcn_raw_buffer_load_b8(scales, lane * 4, (step >> 2) * 256 + (step & 3), 0);
+        }
+    };
+    Tile ahead[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) load(tile0 + d * tile_stride, ahead[d]);
+    W4Group x[S][TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+        const int r = row0 + 16 * t + (lane & 15);  // rows past the last repeat it: their columns of the result are not stored
+        const long row = r < a.rows ? r : a.rows - 1;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int g = (slice * S + s) * 4 + q;
+            x[s][t] = w4_load_x<FP8>(a, row, g, g < k_groups);
+        }
+    }
+    for (int turn = 0; turn < turns; turn += DEPTH) {  // the same for every wave
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (turn + d >= turns) break;
+            const long tile = tile0 + (turn + d) * tile_stride;
+            v4f32 acc[TT];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[t] = v4f32{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const float scale = __uint_as_float(ahead[d].scales[s] << 23);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v8bf wide = w4_widen(ahead[d].codes[s][i], scale);
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, x[s][t].part[i], acc[t], 0, 0, 0);
+                }
+            }
+            load(tile + DEPTH * tile_stride, ahead[d]);
+            float (*mine)[TT][256] = sums[(turn + d) & 1];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) *reinterpret_cast<v4f32*>(&mine[wave][t][(lane & 15) * 16 + 4 * q]) = acc[t];
+            __syncthreads();
+            for (int i = threadIdx.x; i < groups * TT * 256; i += blockDim.x) {
+                const int g = i / (TT * 256), t = i / 256 % TT, cell = i % 256;
+                float s = mine[g * slices][t][cell];
+                for (int w = 1; w < slices; ++w) s += mine[g * slices + w][t][cell];
+                const long r = row0 + 16 * t + cell / 16;
+                const long c = (long(blockIdx.x) * groups + g + (turn + d) * tile_stride) * 16 + cell % 16;
+                if (r >= a.rows || c >= a.w.n) continue;
+                if (a.y_bf16) static_cast<uint16_t*>(a.y)[r * a.y_pitch + c] = uint16_t(bf16_rne_nan(s));
+                else static_cast<float*>(a.y)[r * a.y_pitch + c] = s;
+            }
+        }
+    }
+}
+
 // A workgroup of eight waves takes one tile of sixteen columns and 16 * TT rows; the waves take the tile's quads of k-steps
 // in turn and their sums meet in LDS, in wave order.
 template <int TT, bool FP8>
