@@ -71,6 +71,8 @@ struct m26c_w4 {
 
 namespace {
 
+constexpr long kPitchMost = 1L << 24;  // a kernel addresses up to 32 rows of x or y with 31 bits
+
 int fail(char* err, size_t errlen, int rc, const char* what) {
     if (err && errlen) snprintf(err, errlen, "%s", what);
     return rc;
@@ -83,50 +85,43 @@ void release(m26c_w4* w) {
     delete w;
 }
 
-// Rows that stay in registers: up to 32 rows, k up to 8192 (4096 for more than 16 rows). False if they do not fit.
-template <int TT, int S, int DEPTH>
-int launch_resident(const W4Args& a, bool fp8, hipStream_t st) {
-    const int slices = (a.w.steps + S - 1) / S, groups = 8 / slices, tiles = (a.w.tiles + groups - 1) / groups;
-    constexpr int kWorkgroups = 256;
-    const int turns = (tiles + kWorkgroups - 1) / kWorkgroups, wide = (tiles + turns - 1) / turns;
-    const dim3 grid(unsigned(wide), 1), block(unsigned(64 * slices * groups));
-    if (fp8) w4_resident_kernel<TT, S, DEPTH, true><<<grid, block, 0, st>>>(a, slices, groups, turns);
-    else w4_resident_kernel<TT, S, DEPTH, false><<<grid, block, 0, st>>>(a, slices, groups, turns);
+template <int TT, int S, int W>
+int launch_resident(const W4Args& a, int workgroups, int share, hipStream_t st) {
+    const int slices = (a.w.steps + S - 1) / S, groups = W / slices, tiles = (a.w.tiles + groups - 1) / groups;
+    const int turns = (tiles + workgroups - 1) / workgroups, wide = (tiles + turns - 1) / turns;
+    const dim3 grid(unsigned(wide), unsigned((a.rows + share - 1) / share)), block(64, unsigned(slices), unsigned(groups));
+    if (a.y_bf16) w4_resident_kernel<TT, S, W, uint16_t><<<grid, block, 0, st>>>(a, slices, groups, turns, share);
+    else w4_resident_kernel<TT, S, W, float><<<grid, block, 0, st>>>(a, slices, groups, turns, share);
     return launched();
 }
-template <int TT>
-bool resident(const W4Args& a, bool fp8, hipStream_t st, int& rc) {
-    const int steps = a.w.steps;
-    if (steps <= 8) rc = launch_resident<TT, 1, 4>(a, fp8, st);
-    else if (steps <= 16) rc = launch_resident<TT, 2, 4>(a, fp8, st);
-    else if (steps <= 24) rc = launch_resident<TT, 3, 3>(a, fp8, st);
-    else if (steps <= 32) rc = launch_resident<TT, 4, 3>(a, fp8, st);
-    else if (TT == 1 && steps <= 48) rc = launch_resident<1, 6, 2>(a, fp8, st);
-    else if (TT == 1 && steps <= 64) rc = launch_resident<1, 8, 2>(a, fp8, st);
-    else return false;
-    return true;
-}
 
-template <int TT>
-int launch_w4(const W4Args& args, bool fp8, hipStream_t st) {
-    constexpr long kMost = 65535L * 16 * TT;  // rows of one launch
-    for (long done = 0; done < args.rows; done += kMost) {
-        W4Args a = args;
-        const long n = args.rows - done < kMost ? args.rows - done : kMost;
-        a.rows = int(n);
-        if (fp8) {
-            a.x_codes += done * a.x_pitch;
-            a.x_scales += done * a.x_scales_pitch;
-        } else {
-            a.x += done * a.x_pitch;
-        }
-        a.y = static_cast<char*>(a.y) + done * a.y_pitch * (a.y_bf16 ? 2 : 4);
-        const dim3 grid(unsigned(a.w.tiles), unsigned((n + 16 * TT - 1) / (16 * TT)));
-        if (fp8) w4_matvec_kernel<TT, true><<<grid, 512, 0, st>>>(a);
-        else w4_matvec_kernel<TT, false><<<grid, 512, 0, st>>>(a);
-        if (int rc = launched()) return rc;
+// The form of a product, by sizes alone (us a pass):
+//  * few tiles and rows: a workgroup per tile, rows streamed with the weights. Up to three workgroups per compute unit: 256 tiles
+//    x 32 steps, 1 row 3.9 against 4.9 with resident rows; 626 x 17, 4 rows 5.2 against 6.0; 1024 x 32, 16 rows 10.6
+//    against 9.7 the other way. Also where k is past what registers hold (64 steps).
+//  * otherwise resident rows: sixteen a workgroup, or 32 where a wave's slice of them fits (1024 tiles x 32 steps, 64 rows: 17.8
+//    against 22.3), one workgroup per compute unit over all row runs, so that each loads its rows once.
+//    Sixteen waves hold up to 64 steps (8192 tiles x 32 steps: 48.3 us with sixteen waves of two steps, 50.1 with eight of four);
+//    up to sixteen steps eight waves do, twice as many workgroups up to eight steps (2048 x 8: 7.8 against 8.9).
+int launch_w4(const W4Args& a, hipStream_t st) {
+    const int steps = a.w.steps, runs16 = (a.rows + 15) / 16;
+    if (steps > 64 || long(a.w.tiles) * runs16 <= 768) {
+        const int share = (a.rows + runs16 - 1) / runs16;
+        w4_streamed_kernel<<<dim3(unsigned(a.w.tiles), unsigned(runs16)), 512, 0, st>>>(a, share);
+        return launched();
     }
-    return 0;
+    const int runs = a.rows > 16 && steps <= 32 ? (a.rows + 31) / 32 : runs16, share = (a.rows + runs - 1) / runs;
+    const int workgroups = runs < 256 ? 256 / runs : 1;
+    if (share > 16) {
+        if (steps <= 8) return launch_resident<2, 1, 8>(a, 2 * workgroups, share, st);
+        if (steps <= 16) return launch_resident<2, 2, 8>(a, workgroups, share, st);
+        return launch_resident<2, 2, 16>(a, workgroups, share, st);
+    }
+    if (steps <= 8) return launch_resident<1, 1, 8>(a, 2 * workgroups, share, st);
+    if (steps <= 16) return launch_resident<1, 2, 8>(a, workgroups, share, st);
+    if (steps <= 32) return launch_resident<1, 2, 16>(a, workgroups, share, st);
+    if (steps <= 48) return launch_resident<1, 3, 16>(a, workgroups, share, st);
+    return launch_resident<1, 4, 16>(a, workgroups, share, st);
 }
 
 int w4_run(const m26c_w4* w, W4Args a, bool fp8, void* stream) {
@@ -134,17 +129,24 @@ int w4_run(const m26c_w4* w, W4Args a, bool fp8, void* stream) {
     if (a.rows == 0) return 0;
     int device = -1;
     if (hipGetDevice(&device) != hipSuccess || device != w->device) return 1;
-    if (!a.y || a.y_pitch < w->lay.n || !on(a.y, a.y_bf16 ? 2 : 4)) return 1;
+    if (!a.y || a.y_pitch < w->lay.n || a.y_pitch > kPitchMost || !on(a.y, a.y_bf16 ? 2 : 4)) return 1;
     a.w = w->lay;
+    a.fp8 = fp8;
     a.payload = w->payload;
     a.scales = w->scales;
-    hipStream_t st = hipStream_t(stream);
-    int rc = 0;
-    if (a.rows <= 16 && resident<1>(a, fp8, st, rc)) return rc;
-    if (a.rows > 16 && a.rows <= 32 && resident<2>(a, fp8, st, rc)) return rc;
-    if (a.rows <= 16) return launch_w4<1>(a, fp8, st);
-    if (a.rows <= 32) return launch_w4<2>(a, fp8, st);
-    return launch_w4<4>(a, fp8, st);
+    constexpr int kLaunchRows = 1 << 19;  // row runs are the grid's second dimension
+    for (int left = a.rows;;) {
+        a.rows = left < kLaunchRows ? left : kLaunchRows;
+        if (int rc = launch_w4(a, hipStream_t(stream))) return rc;
+        if ((left -= a.rows) == 0) return 0;
+        if (fp8) {
+            a.x_codes += long(kLaunchRows) * a.x_pitch;
+            a.x_scales += long(kLaunchRows) * a.x_scales_pitch;
+        } else {
+            a.x += long(kLaunchRows) * a.x_pitch;
+        }
+        a.y = static_cast<char*>(a.y) + long(kLaunchRows) * a.y_pitch * (a.y_bf16 ? 2 : 4);
+    }
 }
 
 }  // namespace
@@ -198,7 +200,7 @@ int m26c_block_join(const m26c_join* plan, long rows, const float* h, const uint
 int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, void* stream, m26c_w4** out, char* err, size_t errlen) {
     if (!out) return fail(err, errlen, 1, "w4 weights: no place for the handle");
     *out = nullptr;
-    if (!payload || !scales || n <= 0 || k <= 0 || k % 32 || n > (1L << 26) || k > (1L << 24)) return fail(err, errlen, 1, "w4 weights: bad pointers or sizes");
+    if (!payload || !scales || n <= 0 || k <= 0 || k % 32 || n > kPitchMost || k > kPitchMost) return fail(err, errlen, 1, "w4 weights: bad pointers or sizes");
     if (!on(payload, 16)) return fail(err, errlen, 1, "w4 weights: the payload has to be 16-byte aligned");
     m26c_w4* w = new (std::nothrow) m26c_w4{};
     if (!w) return fail(err, errlen, 2, "w4 weights: out of host memory");
@@ -235,7 +237,7 @@ int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, v
 void m26c_w4_free(m26c_w4* w) { release(w); }
 
 int m26c_w4_matvec(const m26c_w4* w, const uint16_t* x, long x_pitch, int rows, void* y, int y_bf16, long y_pitch, void* stream) {
-    if (rows > 0 && (!w || !x || !on(x, 16) || x_pitch < w->lay.k || x_pitch % 8)) return 1;
+    if (rows > 0 && (!w || !x || !on(x, 16) || x_pitch < w->lay.k || x_pitch > kPitchMost || x_pitch % 8)) return 1;
     W4Args a{};
     a.x = x; a.x_pitch = x_pitch; a.rows = rows; a.y = y; a.y_bf16 = y_bf16 != 0; a.y_pitch = y_pitch;
     return w4_run(w, a, false, stream);
@@ -244,7 +246,7 @@ int m26c_w4_matvec(const m26c_w4* w, const uint16_t* x, long x_pitch, int rows, 
 int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_pitch, const uint8_t* scales, size_t scales_pitch,
                        int rows, void* y, int y_bf16, long y_pitch, void* stream) {
     if (rows > 0 && (!w || !payload || !scales || !on(payload, 8) || payload_pitch % 8 || payload_pitch < size_t(w->lay.k) ||
-                     scales_pitch < size_t(w->lay.k / 32) || payload_pitch > size_t(1) << 40 || scales_pitch > size_t(1) << 40))
+                     scales_pitch < size_t(w->lay.k / 32) || payload_pitch > size_t(kPitchMost) || scales_pitch > size_t(kPitchMost)))
         return 1;
     W4Args a{};
     a.x_codes = payload; a.x_scales = scales; a.x_pitch = long(payload_pitch); a.x_scales_pitch = long(scales_pitch);

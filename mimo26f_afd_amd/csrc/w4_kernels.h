@@ -9,9 +9,10 @@
 // on one of a compute unit's four SIMDs; at 6.5 TB/s such a kilobyte arrives every 96 cycles per compute unit.
 //
 // Operand order. v_mfma_f32_16x16x32_bf16: lane l holds row (l % 16) of either operand, eight k values of quarter
-// (l / 16); the result's lane l holds D[4 * (l / 16) + i][l % 16]. Which k a quarter stands for is free as long as both
-// operands agree: lane l takes group 4 * step + l / 16 of a 128-wide k-step, the 16 code bytes of one group of one weight row
-// as the checkpoint has them, and feeds its 32 values to four MFMAs, eight at a time.
+// (l / 16); the result's lane l holds D[4 * (l / 16) + i][l % 16]. A 128-wide k-step is four MFMAs, one per group of 32, and a
+// quarter is eight neighbouring values: the four lanes of a row of x read 64 neighbouring bytes with each load.
+// (With a quarter holding a whole group the checkpoint's 16 bytes of a group stay together, but a load of x touches 64 separate
+// pieces of 16 bytes: 16 rows x 4096 took 3.4 us to fetch instead of 1.)
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -23,9 +24,9 @@ typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef float v4f32 __attribute__((ext_vector_type(4)));
 
-// Prepared weights. payload [tile = ceil(n / 16)][step = ceil(k / 128)][lane = 64][16 B]; scales [tile][quad =
-// ceil(steps / 4)][lane = 64][4 B], byte b of a dword for step 4 * quad + b. Rows past n and groups past k hold zero
-// codes under scale 1.
+// Prepared weights. payload [tile = ceil(n / 16)][step = ceil(k / 128)][lane = 64][4 dwords]: dword i of lane l is dword
+// l / 16 of group 4 * step + i of row 16 * tile + l % 16 (eight codes, low nibble first). scales [tile][quad = ceil(steps / 4)]
+// [column = 16][step % 4][4 B], byte i for group i of the step. Rows past n and groups past k hold zero codes under scale 1.
 struct W4Layout {
     long n, k;
     int tiles, steps, quads;
@@ -34,21 +35,30 @@ struct W4Layout {
 __global__ void __launch_bounds__(256) w4_prepare_kernel(const uint8_t* __restrict__ payload, const uint8_t* __restrict__ scales, W4Layout w,
                                                          uint8_t* __restrict__ out, uint8_t* __restrict__ out_scales, uint32_t* __restrict__ fault) {
     const long cells = long(w.tiles) * w.quads * 4 * 64;  // one lane of one step, the last quad's missing steps included
-    for (long i = long(blockIdx.x) * 256 + threadIdx.x; i < cells; i += long(gridDim.x) * 256) {
-        const int lane = int(i & 63);
-        const long step = (i >> 6) % (w.quads * 4), tile = (i >> 6) / (w.quads * 4);
-        const long row = tile * 16 + (lane & 15), group = step * 4 + (lane >> 4), groups = w.k / 32;
-        uint4 codes = make_uint4(0, 0, 0, 0);
+    for (long cell = long(blockIdx.x) * 256 + threadIdx.x; cell < cells; cell += long(gridDim.x) * 256) {
+        const int lane = int(cell & 63), q = lane >> 4;
+        const long step = (cell >> 6) % (w.quads * 4), tile = (cell >> 6) / (w.quads * 4);
+        const long row = tile * 16 + (lane & 15), groups = w.k / 32;
+        const long group = step * 4 + q;  // this lane reads group q of its row's step and takes care of its scale
+        uint4 all = make_uint4(0, 0, 0, 0);
         uint32_t s = 127;
         if (row < w.n && group < groups) {
-            codes = *reinterpret_cast<const uint4*>(payload + row * (w.k / 2) + group * 16);
-            if ((codes.x | codes.y | codes.z | codes.w) & 0x77777777u) {
+            all = *reinterpret_cast<const uint4*>(payload + row * (w.k / 2) + group * 16);
+            if ((all.x | all.y | all.z | all.w) & 0x77777777u) {
                 s = scales[row * groups + group];
                 if (s < 2 || s > 252) { atomicOr(fault, 1u); s = 127; }
             }
         }
-        if (step < w.steps) *reinterpret_cast<uint4*>(out + ((tile * w.steps + step) * 64 + lane) * 16) = codes;
-        out_scales[((tile * w.quads + step / 4) * 64 + lane) * 4 + step % 4] = uint8_t(s);
+        // dword i of this lane is dword q of the lane that read group i: the four lanes of a row exchange in four rounds
+        uint32_t dword[4];
+        for (int d = 0; d < 4; ++d) {
+            const int other = q ^ d;
+            const uint32_t got = __shfl_xor(other == 0 ? all.x : other == 1 ? all.y : other == 2 ? all.z : all.w, 16 * d);
+            for (int i = 0; i < 4; ++i)
+                if (i == other) dword[i] = got;
+        }
+        if (step < w.steps) *reinterpret_cast<uint4*>(out + ((tile * w.steps + step) * 64 + lane) * 16) = make_uint4(dword[0], dword[1], dword[2], dword[3]);
+        out_scales[(((tile * w.quads + step / 4) * 16 + (lane & 15)) * 4 + step % 4) * 4 + q] = uint8_t(s);
     }
 }
 
@@ -59,6 +69,7 @@ struct W4Args {
     const uint16_t* x;       // BF16 rows, or
     const uint8_t* x_codes;  // wire rows
     const uint8_t* x_scales;
+    bool fp8;
     long x_pitch;            // elements, or bytes of the codes
     long x_scales_pitch;
     int rows;
@@ -77,46 +88,7 @@ __device__ __forceinline__ v8bf w4_widen(uint32_t codes, float scale) {
     return u.all;
 }
 
-// The 32 values of one group of one row of x, as four MFMA operands.
-struct W4Group {
-    v8bf part[4];
-};
-template <bool FP8>
-__device__ __forceinline__ W4Group w4_load_x(const W4Args& a, long row, long group, bool there) {
-    W4Group g;
-    if (!there) {  // past k: the weights are zero there, x has to be a number
-        for (int i = 0; i < 4; ++i) g.part[i] = v8bf{};
-        return g;
-    }
-    if constexpr (FP8) {
-        const uint8_t* p = a.x_codes + row * a.x_pitch + group * 32;
-        const uint32_t s = a.x_scales[row * a.x_scales_pitch + group];
-        // scale byte 0 marks a block of zeros; 255 is not a number, and a NaN scale makes every product one
-        const float scale = __uint_as_float(s == 255u ? 0x7fc00000u : (s ? s : 1u) << 23);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint2 c = *reinterpret_cast<const uint2*>(p + 8 * i);
-            union { v2bf pair[4]; v8bf all; } u;
-            u.pair[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, scale, false);
-            u.pair[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.x, scale, true);
-            u.pair[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, scale, false);
-            u.pair[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.y, scale, true);
-            if (s == 255u)
-                for (int j = 0; j < 8; ++j) u.all[j] = __bf16(__builtin_nanf(""));
-            g.part[i] = u.all;
-        }
-    } else {
-        const uint16_t* p = a.x + row * a.x_pitch + group * 32;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            union { uint4 bits; v8bf all; } u;
-            u.bits = *reinterpret_cast<const uint4*>(p + 8 * i);
-            g.part[i] = u.all;
-        }
-    }
-    return g;
-}
-
+typedef uint32_t v2u32 __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u32 __attribute__((ext_vector_type(4)));
 
 // A run of memory with its end: loads past it return zero and move nothing, so a wave may ask for steps or tiles that are
@@ -124,140 +96,215 @@ typedef uint32_t v4u32 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_run_of(const void* base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, bytes, 0x00027000);
 }
+constexpr uint32_t kRunMost = 0x7fffffff;  // a run whose end only kOutside passes
+constexpr int kOutside = int(0x80000000u);
 constexpr int kStreamed = 2;  // non-temporal: a weight is used once
 
+// A lane's share of STEPS k-steps of TT * 16 rows of x, as MFMA operands. The operand order asks for 64 bytes of each of
+// sixteen rows at a time, which a compute unit's memory path serves at 16 bytes a cycle; four rows of 256 bytes come at
+// 40 to 52. So a wave loads whole steps of rows, 256 bytes (128 of wire rows) each, and turns them round in a corner of LDS
+// of its own. All loads are issued before the first is looked at; what is past k or past the last row is asked for outside the
+// buffer, which moves nothing and gives zero. (Past k the weights are zero and x has to be a number.)
+constexpr int kTurnRow = 256 + 16, kTurnBytes = 16 * kTurnRow;  // a row's step in LDS, padded so that the rows of a column start in different banks
+template <int STEPS, int TT>
+struct W4Rows {
+    v8bf part[STEPS][TT][4];
+
+    __device__ __forceinline__ void load(const W4Args& a, long row0, int rows, int step0, uint8_t* corner) {
+        const int lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
+        if (a.fp8) {
+            const __amdgpu_buffer_rsrc_t codes = w4_run_of(a.x_codes + row0 * a.x_pitch, kRunMost);
+            const __amdgpu_buffer_rsrc_t bytes = w4_run_of(a.x_scales + row0 * a.x_scales_pitch, kRunMost);
+            v2u32 raw[STEPS][TT][4];
+            uint32_t scale[STEPS][TT][4];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 16 * t + 4 * i + q, group = (step0 + s) * 4 + i;
+                        const bool there = row < rows && (step0 + s) * 128 + c * 8 < a.w.k, group_there = 16 * t + c < rows && group * 32 < a.w.k;
+                        raw[s][t][i] = __builtin_amdgcn_raw_buffer_load_b64(codes, there ? row * int(a.x_pitch) + c * 8 : kOutside, (step0 + s) * 128, 0);
+                        scale[s][t][i] = __builtin_amdgcn_raw_buffer_load_b8(bytes, group_there ? (16 * t + c) * int(a.x_scales_pitch) : kOutside, group, 0);
+                    }
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<v2u32*>(corner + (4 * i + q) * kTurnRow + c * 8) = raw[s][t][i];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const v2u32 code = *reinterpret_cast<const v2u32*>(corner + c * kTurnRow + i * 32 + q * 8);
+                        const uint32_t byte = scale[s][t][i];
+                        const float f = __uint_as_float((byte ? byte : 1u) << 23);  // byte 0 marks a block of zeros
+                        union { v2bf pair[4]; v8bf all; uint32_t dword[4]; } u;
+                        u.pair[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code.x, f, false);
+                        u.pair[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code.x, f, true);
+                        u.pair[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code.y, f, false);
+                        u.pair[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code.y, f, true);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) u.dword[j] = byte == 255u ? 0x7fc07fc0u : u.dword[j];  // 255 is not a number
+                        part[s][t][i] = u.all;
+                    }
+                }
+        } else {
+            const __amdgpu_buffer_rsrc_t x = w4_run_of(a.x + row0 * a.x_pitch, kRunMost);
+            v4u32 raw[STEPS][TT][4];
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 16 * t + 4 * i + q;
+                        const bool there = row < rows && (step0 + s) * 128 + c * 8 < a.w.k;
+                        raw[s][t][i] = __builtin_amdgcn_raw_buffer_load_b128(x, there ? row * int(a.x_pitch) * 2 + c * 16 : kOutside, (step0 + s) * 256, 0);
+                    }
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u32*>(corner + (4 * i + q) * kTurnRow + c * 16) = raw[s][t][i];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) part[s][t][i] = *reinterpret_cast<const v8bf*>(corner + c * kTurnRow + i * 64 + q * 16);
+                }
+        }
+    }
+};
+
+// The scale of group i of a step out of the step's dword.
+__device__ __forceinline__ float w4_scale(uint32_t dword, int i) { return __uint_as_float((dword >> (8 * i) & 0xffu) << 23); }
+
 // Rows resident: x stays in registers. A workgroup's waves are `groups` column groups of `slices` k-slices, S steps each;
-// a wave converts its slice of 16 * TT rows to matrix operands once and then walks over tiles, DEPTH of them in flight, with
-// nothing but weights left to load. The slices' sums meet in LDS, in order, two buffers taking turns so that one
-// barrier per tile does.
-template <int TT, int S, int DEPTH, bool FP8>
-__global__ void __launch_bounds__(512) w4_resident_kernel(const W4Args a, int slices, int groups, int turns) {
-    __shared__ float sums[2][8][TT][256];
-    const int lane = threadIdx.x & 63, q = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slice = wave % slices, group = wave / slices;
-    const int row0 = blockIdx.y * 16 * TT, k_groups = int(a.w.k / 32);
-    const long tile0 = long(blockIdx.x) * groups + group, tile_stride = long(gridDim.x) * groups;
+// a wave converts its slice of 16 * TT rows to matrix operands once and then walks over the tiles, DEPTH of them in flight,
+// with nothing but weights left to load. The slices' sums meet in LDS, in order, two buffers taking turns so that one
+// barrier per turn does. A workgroup's tiles are neighbours, so that what it writes of a row grows into whole 256-byte
+// pieces in its L2 (16 rows x 131072 columns from 131072 x 4096: 50 us; with a workgroup's tiles a grid apart, 64 bytes
+// of a row from each XCD in turn, 55). Tiles past the last load and store nothing. blockIdx.y is a run of `share` rows.
+template <int TT, int S, int W, typename OUT>
+__global__ void __launch_bounds__(64 * W, W / 4) w4_resident_kernel(const W4Args a, int slices, int groups, int turns, int share) {
+    // Each wave's corner while x is turned round, the slices' sums afterwards.
+    constexpr int kSums = 2 * W * TT * 256 * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t shared[kSums > W * kTurnBytes ? kSums : W * kTurnBytes];
+    float (*sums)[W][TT][256] = reinterpret_cast<float (*)[W][TT][256]>(shared);
+    // a workgroup is (64 lanes, slices, groups)
+    const int lane = threadIdx.x, q = lane >> 4;
+    const int slice = __builtin_amdgcn_readfirstlane(threadIdx.y), group = __builtin_amdgcn_readfirstlane(threadIdx.z), wave = group * slices + slice;
+    const int row0 = blockIdx.y * share, rows = a.rows - row0 < share ? a.rows - row0 : share, threads = groups * slices * 64;
+    auto tile_of = [&](int turn) { return turn < turns ? (int(blockIdx.x) * turns + turn) * groups : a.w.tiles; };  // of column group 0
     const uint32_t step_bytes = uint32_t(a.w.steps) * 1024, scale_bytes = uint32_t(a.w.quads) * 256;
     struct Tile {
         v4u32 codes[S];
         uint32_t scales[S];
     };
-    auto load = [&](long tile, Tile& t) {
+    auto load = [&](int tile, Tile& t) {
         const bool there = tile < a.w.tiles;
         const long at = there ? tile : 0;
         const __amdgpu_buffer_rsrc_t codes = w4_run_of(a.payload + at * step_bytes, there ? step_bytes : 0);
         const __amdgpu_buffer_rsrc_t scales = w4_run_of(reinterpret_cast<const uint8_t*>(a.scales) + at * scale_bytes, there ? scale_bytes : 0);
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int step = slice * S + s;
-            t.codes[s] = __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, step * 1024, kStreamed);
-            // one byte per step and lane; four neighbouring steps share a dword
-            t.scales[s] = __builtin_amdgcn_raw_buffer_load_b8(scales, lane * 4, (step >> 2) * 256 + (step & 3), 0);
-        }
-    };
-    Tile ahead[DEPTH];
+        for (int s = 0; s < S; ++s) t.codes[s] = __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, (slice * S + s) * 1024, kStreamed);
+        // a dword per step and column; four steps of a quad lie together
+        if constexpr (S % 4 == 0) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(tile0 + d * tile_stride, ahead[d]);
-    W4Group x[S][TT];
+            for (int s = 0; s < S; s += 4) {
+                const v4u32 v = __builtin_amdgcn_raw_buffer_load_b128(scales, (lane & 15) * 16, (slice * S + s) * 64, kStreamed);
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        const int r = row0 + 16 * t + (lane & 15);  // rows past the last repeat it: their columns of the result are not stored
-        const long row = r < a.rows ? r : a.rows - 1;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int g = (slice * S + s) * 4 + q;
-            x[s][t] = w4_load_x<FP8>(a, row, g, g < k_groups);
-        }
-    }
-    for (int turn = 0; turn < turns; turn += DEPTH) {  // the same for every wave
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            if (turn + d >= turns) break;
-            const long tile = tile0 + (turn + d) * tile_stride;
-            v4f32 acc[TT];
-#pragma unroll
-            for (int t = 0; t < TT; ++t) acc[t] = v4f32{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < 4; ++j) t.scales[s + j] = v[j];
+            }
+        } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const float scale = __uint_as_float(ahead[d].scales[s] << 23);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const v8bf wide = w4_widen(ahead[d].codes[s][i], scale);
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, x[s][t].part[i], acc[t], 0, 0, 0);
-                }
+                const int step = slice * S + s;
+                t.scales[s] = __builtin_amdgcn_raw_buffer_load_b32(scales, (lane & 15) * 16, (step >> 2) * 256 + (step & 3) * 4, kStreamed);
             }
-            load(tile + DEPTH * tile_stride, ahead[d]);
-            float (*mine)[TT][256] = sums[(turn + d) & 1];
+        }
+    };
+    Tile ahead;
+    load(tile_of(0) + group, ahead);
+    W4Rows<S, TT> x;
+    x.load(a, row0, rows, slice * S, shared + wave * kTurnBytes);
+    __syncthreads();
+    for (int turn = 0; turn < turns; ++turn) {  // the same for every wave
+        const int tile = tile_of(turn);
+        v4f32 acc[TT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) *reinterpret_cast<v4f32*>(&mine[wave][t][(lane & 15) * 16 + 4 * q]) = acc[t];
-            __syncthreads();
-            for (int i = threadIdx.x; i < groups * TT * 256; i += blockDim.x) {
-                const int g = i / (TT * 256), t = i / 256 % TT, cell = i % 256;
-                float s = mine[g * slices][t][cell];
-                for (int w = 1; w < slices; ++w) s += mine[g * slices + w][t][cell];
-                const long r = row0 + 16 * t + cell / 16;
-                const long c = (long(blockIdx.x) * groups + g + (turn + d) * tile_stride) * 16 + cell % 16;
-                if (r >= a.rows || c >= a.w.n) continue;
-                if (a.y_bf16) static_cast<uint16_t*>(a.y)[r * a.y_pitch + c] = uint16_t(bf16_rne_nan(s));
-                else static_cast<float*>(a.y)[r * a.y_pitch + c] = s;
+        for (int t = 0; t < TT; ++t) acc[t] = v4f32{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const v8bf wide = w4_widen(ahead.codes[s][i], w4_scale(ahead.scales[s], i));
+#pragma unroll
+                for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, x.part[s][t][i], acc[t], 0, 0, 0);
+            }
+        load(tile_of(turn + 1) + group, ahead);  // under the sums and stores of this one
+        float (*mine)[TT][256] = sums[turn & 1];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) *reinterpret_cast<v4f32*>(&mine[wave][t][(lane & 15) * 16 + 4 * q]) = acc[t];
+        __syncthreads();
+        const __amdgpu_buffer_rsrc_t y = w4_run_of(static_cast<OUT*>(a.y) + row0 * a.y_pitch + long(tile) * 16, kRunMost);
+        const long left = a.w.n - long(tile) * 16;
+        for (int i = wave * 64 + lane; i < groups * TT * 256; i += threads) {
+            const int g = i / (TT * 256), t = i / 256 % TT, cell = i % 256, r = 16 * t + cell / 16, c = 16 * g + cell % 16;
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const float part = mine[g * slices + (w < slices ? w : 0)][t][cell];
+                s += w < slices ? part : 0.0f;
+            }
+            const int at = (r * int(a.y_pitch) + c) * int(sizeof(OUT));
+            if (r < rows && c < left) {
+                if constexpr (sizeof(OUT) == 2) __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bf16_rne_nan(s)), y, at, 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s), y, at, 0, 0);
             }
         }
     }
 }
 
-// A workgroup of eight waves takes one tile of sixteen columns and 16 * TT rows; the waves take the tile's quads of k-steps
-// in turn and their sums meet in LDS, in wave order.
-template <int TT, bool FP8>
-__global__ void __launch_bounds__(512) w4_matvec_kernel(const W4Args a) {
+// Rows streamed: a workgroup of eight waves takes one tile of sixteen columns and `share` <= 16 rows; the waves take the
+// tile's quads of k-steps in turn, weights and rows alike, and their sums meet in LDS, in wave order. A step at a time: with a
+// quad's sixteen loads of x ahead of its products a wave holds twice the registers, and where two or three tiles meet on a
+// compute unit that costs more than it hides (626 tiles x 17 steps 8.5 against 6.6 us, 256 x 32 4.0 against 3.9).
+__global__ void __launch_bounds__(512) w4_streamed_kernel(const W4Args a, int share) {
     constexpr int WAVES = 8;
-    __shared__ float sums[WAVES][TT][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
-    const long tile = blockIdx.x, row0 = long(blockIdx.y) * 16 * TT, groups = a.w.k / 32;
-    v4f32 acc[TT];
-    long row[TT];  // rows past the last repeat it: their columns of the result are not stored
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        acc[t] = v4f32{0.f, 0.f, 0.f, 0.f};
-        const long r = row0 + 16 * t + (lane & 15);
-        row[t] = r < a.rows ? r : a.rows - 1;
-    }
+    __shared__ float sums[WAVES][256];
+    __shared__ __attribute__((aligned(16))) uint8_t corners[WAVES][kTurnBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
+    const long tile = blockIdx.x, row0 = long(blockIdx.y) * share;
+    const int rows = a.rows - row0 < share ? int(a.rows - row0) : share;
     const uint4* payload = reinterpret_cast<const uint4*>(a.payload) + tile * a.w.steps * 64 + lane;
-    const uint32_t* scales = a.scales + tile * a.w.quads * 64 + lane;
+    const uint4* scales = reinterpret_cast<const uint4*>(a.scales) + tile * a.w.quads * 16 + (lane & 15);
+    v4f32 acc = {0.f, 0.f, 0.f, 0.f};
     for (int quad = wave; quad < a.w.quads; quad += WAVES) {
-        const uint32_t sc = scales[quad * 64];
+        const uint4 four = scales[quad * 16];
+        const uint32_t scale[4] = {four.x, four.y, four.z, four.w};
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int step = quad * 4 + b;
+        for (int s = 0; s < 4; ++s) {
+            const int step = quad * 4 + s;
             if (step >= a.w.steps) break;  // the same for the whole workgroup
             const uint4 codes = payload[step * 64];
-            const long group = long(step) * 4 + q;
-            W4Group x[TT];
-#pragma unroll
-            for (int t = 0; t < TT; ++t) x[t] = w4_load_x<FP8>(a, row[t], group, group < groups);
-            const float scale = __uint_as_float(((sc >> (8 * b)) & 0xffu) << 23);
             const uint32_t dword[4] = {codes.x, codes.y, codes.z, codes.w};
+            W4Rows<1, 1> x;
+            x.load(a, row0, rows, step, corners[wave]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const v8bf wide = w4_widen(dword[i], scale);
-#pragma unroll
-                for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, x[t].part[i], acc[t], 0, 0, 0);
-            }
+            for (int i = 0; i < 4; ++i)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w4_widen(dword[i], w4_scale(scale[s], i)), x.part[0][0][i], acc, 0, 0, 0);
         }
     }
-#pragma unroll
-    for (int t = 0; t < TT; ++t)  // [row][column of the tile]
-        *reinterpret_cast<v4f32*>(&sums[wave][t][(lane & 15) * 16 + 4 * q]) = acc[t];
+    *reinterpret_cast<v4f32*>(&sums[wave][(lane & 15) * 16 + 4 * q]) = acc;  // [row][column of the tile]
     __syncthreads();
-    for (int i = threadIdx.x; i < TT * 256; i += 512) {
-        const long r = row0 + i / 16, c = tile * 16 + i % 16;
-        float s = sums[0][i / 256][i % 256];
+    const int i = threadIdx.x, r = i / 16;
+    const long c = tile * 16 + i % 16;
+    if (i >= 256 || r >= rows || c >= a.w.n) return;
+    float s = sums[0][i];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) s += sums[w][i / 256][i % 256];
-        if (r >= a.rows || c >= a.w.n) continue;
-        if (a.y_bf16) static_cast<uint16_t*>(a.y)[r * a.y_pitch + c] = uint16_t(bf16_rne_nan(s));
-        else static_cast<float*>(a.y)[r * a.y_pitch + c] = s;
-    }
+    for (int w = 1; w < WAVES; ++w) s += sums[w][i];
+    if (a.y_bf16) static_cast<uint16_t*>(a.y)[(row0 + r) * a.y_pitch + c] = uint16_t(bf16_rne_nan(s));
+    else static_cast<float*>(a.y)[(row0 + r) * a.y_pitch + c] = s;
 }
 
 }  // namespace m26g

@@ -218,7 +218,10 @@ def run_w4(weights, x, rows, fp8=None, bf16_out=False, x_pad=0, y_pad=0):
 
 
 SHAPES = [(1, 1, 32), (1, 16, 64), (3, 17, 96), (16, 256, 4096), (17, 100, 128), (5, 1000, 2080), (33, 48, 160), (64, 130, 512), (65, 40, 544), (130, 31, 1024),
-          (1, 4096, 4096), (2, 5, 16384), (48, 4099, 608), (16, 33000, 256)]
+          (1, 4096, 4096), (2, 5, 16384), (48, 4099, 608), (16, 33000, 256),
+          # every form of the rule on sizes: steps of 128 up to 8, 16, 24, 32, 48, 64 and more, in runs of 16 and 32 rows, tiles past one turn
+          (3, 13000, 1056), (16, 12500, 2080), (9, 12400, 3200), (7, 12400, 4128), (5, 12330, 6176), (2, 12330, 8224), (33, 8200, 96), (29, 13000, 1056),
+          (64, 8200, 2080), (50, 4200, 3200), (64, 4200, 4128), (300, 200, 640), (2, 40, 16416)]
 
 
 @pytest.mark.parametrize("rows,n,k", SHAPES)
@@ -336,6 +339,8 @@ def test_w4_refuses_calls_that_do_not_fit():
            lambda: weights.matvec(None, 1, y.ptr), lambda: weights.matvec(x.ptr, 1, None), lambda: weights.matvec(x.ptr, 1, y.ptr + 1, True),
            lambda: weights.matvec_fp8(x.ptr + 4, x.ptr, 1, y.ptr), lambda: weights.matvec_fp8(x.ptr, x.ptr, 1, y.ptr, payload_pitch=68),
            lambda: weights.matvec_fp8(x.ptr, None, 1, y.ptr), lambda: weights.matvec_fp8(x.ptr, x.ptr, 1, y.ptr, scales_pitch=1)]
+    bad += [lambda: weights.matvec(x.ptr, 2, y.ptr, x_pitch=1 << 25), lambda: weights.matvec(x.ptr, 2, y.ptr, y_pitch=(1 << 24) + 1),
+            lambda: weights.matvec_fp8(x.ptr, x.ptr, 2, y.ptr, payload_pitch=1 << 25)]
     for call in bad:
         with pytest.raises(coord.CoordError) as e:
             call()
