@@ -23,40 +23,48 @@ void launch_join(const JoinArgs& a, bool vec, unsigned grid, hipStream_t st) {
 }
 
 // ---- log probabilities
-// Segments of a row: enough workgroups for four per compute unit where the rows alone are too few, but at least
-// two chunks for each of a workgroup's waves.
-int segments_of(int rows, int vocab) {
-    const long chunks = (long(vocab) + kChunk - 1) / kChunk;
-    long s = (1024 + rows - 1) / rows;
-    const long most = chunks / (2 * kLogprobWaves);
-    s = s < most ? s : most;
-    s = s < kSegmentsMost ? s : kSegmentsMost;
-    return int(s < 1 ? 1 : s);
+// Parts of a row, 0 where a workgroup takes whole rows: from 32 rows on there are enough of those.
+constexpr int kRowsWhole = 32;
+int parts_of(int rows, int vocab) {
+    if (rows >= kRowsWhole) return 0;
+    const int chunks = vocab / kChunk;
+    const int parts = chunks / 2 / kPartWaves * kPartWaves;  // two chunks to a wave at least
+    const int most = 4096 / rows / kPartWaves * kPartWaves;  // four waves per SIMD over all rows
+    const int p = parts < most ? parts : most;
+    return p <= 16 ? 0 : p < kPartsMost ? p : kPartsMost;  // a workgroup's sixteen waves do as well
 }
-size_t stats_bytes(int rows, int segments) { return size_t(rows) * segments * sizeof(float4); }
+size_t stats_bytes(int rows, int parts) { return size_t(rows) * parts * sizeof(float4); }
+
+template <bool BF16, int WAVES>
+int launch_rows(const LogprobArgs& a, hipStream_t st) {
+    constexpr int kMost = (1 << 25) / (64 * WAVES);  // rows of a launch: it holds under 2^32 threads
+    for (int done = 0; done < a.rows;) {
+        const int n = a.rows - done < kMost ? a.rows - done : kMost;
+        LogprobArgs b = a;
+        b.rows = n;
+        b.logits = static_cast<const char*>(a.logits) + long(done) * a.pitch * (BF16 ? 2 : 4);
+        if (a.n_given) { b.given = a.given + long(done) * a.n_given; b.given_logprob = a.given_logprob + long(done) * a.n_given; }
+        if (a.entropy) b.entropy = a.entropy + done;
+        if (a.top) { b.top_ids = a.top_ids + long(done) * a.top; b.top_logprob = a.top_logprob + long(done) * a.top; }
+        logprob_row_kernel<BF16, WAVES><<<unsigned(n), 64 * WAVES, 0, st>>>(b);
+        if (int rc = launched()) return rc;
+        done += n;
+    }
+    return 0;
+}
 
 template <bool BF16>
-int launch_logprobs(LogprobArgs a, hipStream_t st) {
-    if (a.segments == 1) {
-        const size_t size = BF16 ? 2 : 4;
-        for (int done = 0; done < a.rows;) {  // a launch holds under 2^32 threads
-            const int n = a.rows - done < (1 << 23) ? a.rows - done : (1 << 23);
-            LogprobArgs b = a;
-            b.rows = n;
-            b.logits = static_cast<const char*>(a.logits) + size_t(done) * a.pitch * size;
-            if (a.n_given) { b.given = a.given + size_t(done) * a.n_given; b.given_logprob = a.given_logprob + size_t(done) * a.n_given; }
-            if (a.entropy) b.entropy = a.entropy + done;
-            if (a.top) { b.top_ids = a.top_ids + size_t(done) * a.top; b.top_logprob = a.top_logprob + size_t(done) * a.top; }
-            logprob_kernel<BF16><<<unsigned(n), 64 * kLogprobWaves, 0, st>>>(b);
-            if (int rc = launched()) return rc;
-            done += n;
-        }
-        return 0;
+int launch_logprobs(const LogprobArgs& a, hipStream_t st) {
+    if (a.parts) {
+        logprob_part_kernel<BF16><<<unsigned(a.rows) * unsigned(a.parts / kPartWaves), 64 * kPartWaves, 0, st>>>(a);
+        if (int rc = launched()) return rc;
+        logprob_join_kernel<BF16><<<unsigned(a.rows), 1024, 0, st>>>(a);
+        return launched();
     }
-    logprob_kernel<BF16><<<unsigned(a.rows) * unsigned(a.segments), 64 * kLogprobWaves, 0, st>>>(a);
-    if (int rc = launched()) return rc;
-    logprob_join_kernel<BF16><<<unsigned(a.rows), 256, size_t(a.segments) * a.top * 8, st>>>(a);
-    return launched();
+    const int chunks = a.vocab / kChunk;
+    if (chunks <= 2) return launch_rows<BF16, 1>(a, st);
+    if (a.rows >= 1024 || chunks <= 8) return launch_rows<BF16, 4>(a, st);
+    return launch_rows<BF16, 16>(a, st);
 }
 
 }  // namespace
@@ -256,8 +264,8 @@ int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_
 
 size_t m26c_token_logprobs_workspace(int rows, int vocab, int top) {
     if (rows <= 0 || vocab <= 0 || top < 0 || top > kTopMost) return 0;
-    const int segments = segments_of(rows, vocab);
-    return segments == 1 ? 0 : stats_bytes(rows, segments) + size_t(rows) * segments * top * 8;
+    const int parts = parts_of(rows, vocab);
+    return stats_bytes(rows, parts) + size_t(rows) * parts * top * 8;
 }
 
 int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int vocab, float scale, const int* given, int n_given,
@@ -269,7 +277,7 @@ int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int 
         (top && (!top_ids || !top_logprob || !on(top_ids, 4) || !on(top_logprob, 4))))
         return 1;
     LogprobArgs a{};
-    a.segments = segments_of(rows, vocab);
+    a.parts = parts_of(rows, vocab);
     const size_t need = m26c_token_logprobs_workspace(rows, vocab, top);
     if (need && (!workspace || !on(workspace, 16) || workspace_bytes < need)) return 1;
     a.logits = logits; a.pitch = pitch; a.rows = rows; a.vocab = vocab; a.scale = scale;
@@ -277,7 +285,7 @@ int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int 
     a.top = top; a.top_ids = top_ids; a.top_logprob = top_logprob;
     if (need) {
         a.stats = static_cast<float4*>(workspace);
-        a.lists = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + stats_bytes(rows, a.segments));
+        a.lists = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + stats_bytes(rows, a.parts));
     }
     return bf16 ? launch_logprobs<true>(a, hipStream_t(stream)) : launch_logprobs<false>(a, hipStream_t(stream));
 }

@@ -72,17 +72,18 @@ def w4_product(x, w):
 def logprobs(logits, given, top, scale):
     """Per row: given log probabilities, entropy, top ids, their log probabilities, and a bound for each of the three numbers.
 
-    A term exp(t - m) is off by the roundings of v - m and of its product with scale * log2 e (relative 2 |t - m| U32 and the
-    constant's 2 |t - m| U32) and two of the exponential; a lane adds at most vocab / 256 + 24 terms one after another, and 20
-    joins follow, each of which rescales by a factor that is off like a term. The mean of |t - m| under the distribution is
-    what the first part amounts to in Z."""
+    A term exp(t - m) = 2^d is off by the roundings of scale * log2 e and its constant (relative 2 |t - m| U32), of d (|t - m| U32)
+    and two of the exponential; a lane adds at most vocab / 256 + 40 terms one after another (a row of more than two chunks of
+    512 values is at least four waves' work), and 20 joins follow, each of which rescales by a factor that is off like a term.
+    The mean of |t - m| under the distribution is what the first part amounts to in Z. A log probability is (v - m) scale - ln Z:
+    two roundings of the first part, two of the second, one of the difference."""
     rows, vocab = logits.shape
     x = np.asarray(logits, np.float64)
     t = x * scale
     gl = np.full(given.shape, np.nan)
     ent, ids, lp = np.zeros(rows), np.full((rows, top), -1, np.int64), np.full((rows, top), -np.inf)
     tol_g, tol_h, tol_t = np.zeros(given.shape), np.zeros(rows), np.zeros((rows, top))
-    chain = vocab / 256 + 24 + 20
+    chain = vocab / 256 + 40 + 20
     for r in range(rows):
         row = t[r]
         numbers = np.where(np.isnan(row), -np.inf, row)
@@ -108,13 +109,13 @@ def logprobs(logits, given, top, scale):
         logp = d - lnz
         ent[r] = lnz + mean
         spread = np.sum(np.where(p > 0, p * np.where(np.isfinite(d), d, 0) ** 2, 0))
-        tol_h[r] = z_err * (1 + mean) + (chain + 8) * U32 * mean + 4 * spread * U32 + 4 * U32 * (lnz + mean)
+        tol_h[r] = z_err * (1 + mean) + (chain + 8) * U32 * mean + 4 * spread * U32 + 6 * U32 * (lnz + mean)
         gl[r, inside] = logp[given[r, inside]]
         lp[r, :kept.size] = logp[kept]
 
         def bound(v):
             with np.errstate(invalid="ignore"):
-                b = z_err + U32 * (2 * np.abs(v + lnz) + 2 * lnz + np.abs(v))
+                b = z_err + U32 * (3 * np.abs(v + lnz) + 2 * lnz + 3 * np.abs(v))
             return np.where(np.isfinite(v), b, 0)
         tol_g[r] = bound(np.where(inside, gl[r], 0))
         tol_t[r] = bound(lp[r])
