@@ -23,34 +23,23 @@ void launch_join(const JoinArgs& a, bool vec, unsigned grid, hipStream_t st) {
 }
 
 // ---- log probabilities
-// Parts of a row, 0 where a workgroup takes whole rows: from 32 rows on there are enough of those.
-constexpr int kRowsWhole = 32;
+// Parts of a row over several workgroups, about 4096 waves over all rows and two chunks each at least; 0 where that
+// leaves a row fewer than eight and a workgroup takes whole rows (us a pass: 1 row x 131072 logits 13.2 against 30.6 with a
+// workgroup of eight waves, 37 x 50003 14.6 against 18.4, 300 x 131072 44 against 50).
 int parts_of(int rows, int vocab) {
-    if (rows >= kRowsWhole) return 0;
-    const int chunks = vocab / kChunk;
-    const int parts = chunks / 2 / kPartWaves * kPartWaves;  // two chunks to a wave at least
-    const int most = 4096 / rows / kPartWaves * kPartWaves;  // four waves per SIMD over all rows
-    const int p = parts < most ? parts : most;
-    return p <= 16 ? 0 : p < kPartsMost ? p : kPartsMost;  // a workgroup's sixteen waves do as well
+    int parts = vocab / kChunk / 2;
+    parts = parts < 4096 / rows ? parts : 4096 / rows;
+    parts = parts < kPartsMost ? parts : kPartsMost;
+    parts = parts / kPartWaves * kPartWaves;
+    return parts < 8 ? 0 : parts;
 }
 size_t stats_bytes(int rows, int parts) { return size_t(rows) * parts * sizeof(float4); }
 
 template <bool BF16, int WAVES>
 int launch_rows(const LogprobArgs& a, hipStream_t st) {
-    constexpr int kMost = (1 << 25) / (64 * WAVES);  // rows of a launch: it holds under 2^32 threads
-    for (int done = 0; done < a.rows;) {
-        const int n = a.rows - done < kMost ? a.rows - done : kMost;
-        LogprobArgs b = a;
-        b.rows = n;
-        b.logits = static_cast<const char*>(a.logits) + long(done) * a.pitch * (BF16 ? 2 : 4);
-        if (a.n_given) { b.given = a.given + long(done) * a.n_given; b.given_logprob = a.given_logprob + long(done) * a.n_given; }
-        if (a.entropy) b.entropy = a.entropy + done;
-        if (a.top) { b.top_ids = a.top_ids + long(done) * a.top; b.top_logprob = a.top_logprob + long(done) * a.top; }
-        logprob_row_kernel<BF16, WAVES><<<unsigned(n), 64 * WAVES, 0, st>>>(b);
-        if (int rc = launched()) return rc;
-        done += n;
-    }
-    return 0;
+    const int wide = a.rows < 4096 ? a.rows : 4096;  // workgroups walk over the rows from there on
+    logprob_row_kernel<BF16, WAVES><<<unsigned(wide), 64 * WAVES, 0, st>>>(a);
+    return launched();
 }
 
 template <bool BF16>
@@ -58,13 +47,16 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t st) {
     if (a.parts) {
         logprob_part_kernel<BF16><<<unsigned(a.rows) * unsigned(a.parts / kPartWaves), 64 * kPartWaves, 0, st>>>(a);
         if (int rc = launched()) return rc;
-        logprob_join_kernel<BF16><<<unsigned(a.rows), 1024, 0, st>>>(a);
+        logprob_join_kernel<BF16><<<unsigned(a.rows), kJoinThreads, 0, st>>>(a);
         return launched();
     }
+    // Waves to a row: as few as fill the chip, since each finds its own largest values first (2048 rows x 131072: two waves
+    // 103 us, four 118, eight 133; 1024 x 50003: four 49, two 63).
     const int chunks = a.vocab / kChunk;
-    if (chunks <= 2) return launch_rows<BF16, 1>(a, st);
-    if (a.rows >= 1024 || chunks <= 8) return launch_rows<BF16, 4>(a, st);
-    return launch_rows<BF16, 16>(a, st);
+    if (chunks <= 2 && (a.rows >= 768 || chunks == 0)) return launch_rows<BF16, 1>(a, st);
+    if (a.rows >= 1536) return launch_rows<BF16, 2>(a, st);
+    if (a.rows >= 768 || chunks < 16) return launch_rows<BF16, 4>(a, st);
+    return launch_rows<BF16, 8>(a, st);
 }
 
 }  // namespace

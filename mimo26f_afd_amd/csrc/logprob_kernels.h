@@ -11,8 +11,8 @@
 // at a time, with the top-th of them as a threshold. A value above it is put in its place with one comparison and one shift
 // over the lanes; an equal one need not be: `top` values of its size with lower ids are there. One comparison of each
 // lane's maximum, which the softmax needs anyway, and a scalar branch are the whole cost where nothing qualifies, which after i
-// chunks is all but top / i of them. The waves of a workgroup help each other: what each wave's (top / waves)-th value
-// reaches is a bound that `top` values of the row reach. List entries are 64-bit keys, the value's bits in integer order above the
+// chunks is all but top / i of them. The waves of a workgroup help each other: of the 64 values that they have on show, the
+// largest of each, the top-th largest is a bound that `top` values of the row reach. List entries are 64-bit keys, the value's bits in integer order above the
 // complemented id: a total order, so the result does not depend on who finds what when.
 //
 // A row is cut into parts, a wave each, whose chunks lie side by side. The parts' lists meet in one workgroup: their keys in
@@ -22,7 +22,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <type_traits>
-#include "q0_codec.h"
+#include "join_kernels.h"
 
 namespace m26g {
 
@@ -58,13 +58,18 @@ __device__ __forceinline__ float key_value(uint64_t key) { return order_value(ui
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
     return __builtin_amdgcn_mbcnt_hi(uint32_t(mask >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(mask), 0));
 }
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint64_t o = uint64_t(__shfl_xor(uint32_t(v >> 32), d)) << 32 | __shfl_xor(uint32_t(v), d);
-        v = o > v ? o : v;
-    }
-    return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float max_from(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xf, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {  // as wave_sum
+    v = max_from<0xB1, 0xf>(v);
+    v = max_from<0x4E, 0xf>(v);
+    v = max_from<0x141, 0xf>(v);
+    v = max_from<0x140, 0xf>(v);
+    v = max_from<0x142, 0xa>(v);
+    v = max_from<0x143, 0xc>(v);
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // Running sums of 2^(v c - r), c = scale * log2 e, and of that times its exponent, relative to r = m c rounded to FP32, m the
@@ -95,9 +100,11 @@ struct SoftmaxSums {
         z += e;
         s = __builtin_fmaf(e, fmaxf(d, -300.0f), s);  // a masked value adds 0, not 0 * infinity
     }
-    __device__ __forceinline__ void join_lanes(float c) {  // over the wave, in a fixed order, the same in every lane
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) join(SoftmaxSums{__shfl_xor(m, d), __shfl_xor(z, d), __shfl_xor(s, d)}, c);
+    // Over the wave, the same in every lane: the largest m first, then each lane's sums relative to it, added up in a fixed order.
+    __device__ __forceinline__ void join_lanes(float c) {
+        *this = at(wave_max(m), c);
+        z = wave_sum(z);
+        s = wave_sum(s);
     }
 };
 
@@ -120,75 +127,117 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], int top) 
     return cut;
 }
 
-// A wave's largest keys in descending order, lane i the i-th; kNoKey where there are fewer.
+// Orders what other lanes of this wave have written to LDS before what this lane reads next.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The next number below v; below zero that is the smallest negative one.
+__device__ __forceinline__ float just_below(float v) {
+    const uint32_t o = order_bits(v);
+    return order_value(o - (o == 0x80000000u ? 2 : 1));  // below zero's bits lie those of -0, which counts as zero
+}
+
+// A wave's largest keys in descending order, lane i the i-th; kNoKey where there are fewer. Lanes from `top` on mean nothing.
 template <int WAVES>
 struct TopList {
-    float* shared;  // LDS, one of each wave of the workgroup: its share-th largest value
-    int top, share, wave;
+    uint32_t* shown;         // LDS: of each wave of the workgroup the order bits of its 64 / WAVES largest values, 0 for none
+    uint64_t *batch, *turn;  // LDS, 64 each, this wave's
+    int top, wave;
     uint64_t key = kNoKey;
-    uint64_t floor = kNoKey;       // uniform: a key has to be above this one to matter
-    float threshold = -INFINITY;   // uniform: a value of a later chunk has to be above this one
+    float threshold = -INFINITY;  // uniform: a value has to be above this one to matter
+    bool full = false;            // uniform: `top` keys are there
 
-    __device__ __forceinline__ uint64_t of_lane(uint64_t k, int lane) const {
+    __device__ __forceinline__ static uint64_t of_lane(uint64_t k, int lane) {
         return uint64_t(__builtin_amdgcn_readlane(uint32_t(k >> 32), lane)) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(k), lane));
     }
     __device__ __forceinline__ void insert(uint64_t k) {  // k uniform and new
         const bool above = key > k;
-        const uint64_t mask = __ballot(above);  // the first lanes
-        const uint32_t hi = uint32_t(key >> 32), lo = uint32_t(key);
-        const uint64_t moved = uint64_t(__builtin_amdgcn_update_dpp(0u, hi, 0x138, 0xf, 0xf, false)) << 32 |  // wave_shr:1
-                               uint32_t(__builtin_amdgcn_update_dpp(0u, lo, 0x138, 0xf, 0xf, false));
-        const int place = int(__popcll(mask));
+        const int place = int(__popcll(__ballot(above)));  // the lanes above are the first ones
+        const uint64_t moved = uint64_t(__builtin_amdgcn_update_dpp(0u, uint32_t(key >> 32), 0x138, 0xf, 0xf, false)) << 32 |  // wave_shr:1
+                               uint32_t(__builtin_amdgcn_update_dpp(0u, uint32_t(key), 0x138, 0xf, 0xf, false));
         key = above ? key : int(threadIdx.x & 63) == place ? k : moved;
     }
-    // The floor and the threshold from this list's top-th key and from what the waves have in common.
-    __device__ __forceinline__ void settle() {
-        const uint64_t last = of_lane(key, top - 1);
-        floor = last > floor ? last : floor;
-        if (last != kNoKey) threshold = fmaxf(threshold, key_value(last));
+    // Puts up to 64 new keys, one to a lane, kNoKey for none, in their places: a key's place is the number of larger ones.
+    __device__ __forceinline__ void merge(uint64_t fresh, int n) {
+        const int lane = threadIdx.x & 63;
+        int place = 0, moved = lane;
+        key = lane < top ? key : kNoKey;
+        for (int i = 0; i < n; ++i) {
+            const uint64_t k = of_lane(fresh, i);
+            const bool above = key > k;
+            const int before = int(__popcll(__ballot(above)));  // places that the list's keys take ahead of this one
+            moved += !above;
+            place += (lane == i ? before : 0) + (k > fresh);
+        }
+        turn[lane] = kNoKey;
+        wave_fence();
+        if (key != kNoKey && moved < 64) turn[moved] = key;
+        if (fresh != kNoKey && place < 64) turn[place] = fresh;
+        wave_fence();
+        key = turn[lane];
+        wave_fence();
     }
+    // What the values on show vouch for: `top` values of the row reach it, at any ids, so equal ones still count.
     __device__ __forceinline__ void common() {
-        if constexpr (WAVES > 1) {
-            const int lane = threadIdx.x & 63;
-            float v = __hip_atomic_load(&shared[lane % WAVES], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-#pragma unroll
-            for (int d = 1; d < WAVES; d *= 2) v = fminf(v, __shfl_xor(v, d));
-            const uint32_t bound = __builtin_amdgcn_readfirstlane(order_bits(v));
-            // `top` values reach v, at any ids: equal ones still count
-            if (uint64_t(bound) << 32 > floor && v > -INFINITY) {
-                floor = (uint64_t(bound) << 32) - 1;
-                // the next number below it; below zero's bits lie those of -0, which no value has
-                threshold = fmaxf(threshold, order_value(bound - (bound == 0x80000000u ? 2 : 1)));
-            }
-        }
+        const uint32_t v[1] = {__hip_atomic_load(&shown[threadIdx.x & 63], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)};
+        const uint32_t bound = reached_by<16>(v, top);
+        if (bound > order_bits(-INFINITY)) threshold = fmaxf(threshold, just_below(order_value(bound)));
     }
-    // The slow path of a chunk. Element j of the lane has id `id` + j.
-    __device__ __forceinline__ void take(const float (&v)[8], int id) {
-        common();
-        if (of_lane(key, top - 1) == kNoKey) {
-            // Not `top` values yet: the top-th largest of the lanes' maxima is a bound that `top` values of this chunk reach.
-            float most = -INFINITY;
+    // The slow path of a chunk. Element j of the lane has id `id` + j; `most` is the lane's maximum.
+    __device__ __forceinline__ void take(const float (&v)[8], float most, int id) {
+        const int lane = threadIdx.x & 63;
+        if constexpr (WAVES > 2) {  // two waves gain less than the look costs
+            common();
+            if (!__any(most > threshold)) return;
+        }
+        if (!full) {
+            // Not `top` values yet: what `top` of the lanes' maxima reach, as many values of this chunk do.
+            float largest = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) most = v[j] > most ? v[j] : most;  // a NaN takes no part
-            const uint32_t mine[1] = {order_bits(most)};
+            for (int j = 0; j < 8; ++j) largest = v[j] > largest ? v[j] : largest;  // a NaN takes no part
+            const uint32_t mine[1] = {order_bits(largest)};
             const uint32_t bound = reached_by<16>(mine, top);
-            if (bound > order_bits(-INFINITY) && uint64_t(bound) << 32 > floor) floor = (uint64_t(bound) << 32) - 1;
+            if (bound > order_bits(-INFINITY)) threshold = fmaxf(threshold, just_below(order_value(bound)));
         }
+        // Within the chunk ids are not met in order, so all values above the threshold join, and their keys find the order.
+        int n = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint64_t k = list_key(v[j], id + j);
-            const bool number = v[j] > -INFINITY;
-            for (uint64_t mask = __ballot(number && k > floor); mask;) {
-                const int lane = __ffsll(static_cast<unsigned long long>(mask)) - 1;
-                insert(of_lane(k, lane));
-                settle();
-                mask &= mask - 1;
-                mask &= __ballot(k > floor);
+        for (int j = 0; j < 8; ++j) n += int(__popcll(__ballot(v[j] > threshold)));
+        if (n <= 3) {  // one at a time
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                for (uint64_t mask = __ballot(v[j] > threshold); mask; mask &= mask - 1) {
+                    const int from = __ffsll(static_cast<unsigned long long>(mask)) - 1;
+                    const float one = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[j]), from));
+                    insert(list_key(one, __builtin_amdgcn_readlane(id, from) + j));
+                }
+        } else {  // up to 64 at a time
+            n = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool wanted = v[j] > threshold;
+                const uint64_t mask = __ballot(wanted);
+                if (n + int(__popcll(mask)) > 64) {
+                    wave_fence();
+                    merge(lane < n ? batch[lane] : kNoKey, n);
+                    n = 0;
+                }
+                if (wanted) batch[n + lanes_below(mask)] = list_key(v[j], id + j);
+                n += int(__popcll(mask));
             }
+            wave_fence();
+            merge(lane < n ? batch[lane] : kNoKey, n);
         }
-        if constexpr (WAVES > 1) {
-            const uint64_t mine = of_lane(key, share - 1);
-            if (mine != kNoKey && (threadIdx.x & 63) == 0) __hip_atomic_store(&shared[wave], key_value(mine), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        const uint32_t last = __builtin_amdgcn_readlane(uint32_t(key >> 32), top - 1);
+        if (last) {
+            full = true;
+            threshold = fmaxf(threshold, order_value(last));
+        }
+        if constexpr (WAVES > 2) {
+            constexpr int kShow = 64 / WAVES;
+            if (lane < kShow && lane < top) __hip_atomic_store(&shown[wave * kShow + lane], uint32_t(key >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         }
     }
 };
@@ -236,72 +285,95 @@ struct RowPart {
         }
     }
 
+    // Everything but what the whole chunks of ordinary rows need: element by element, with comparisons for the maximum (the
+    // hardware's passes a signalling NaN on, quieted, and loses what it was compared with) and any size of values.
+    template <typename LIST>
+    __device__ __forceinline__ void slowly(const LogprobArgs& a, SoftmaxSums& sum, LIST& list, int id, int stop, float c) const {
+        float v[8], most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = id + j < stop ? value(id + j) : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = v[j] > most ? v[j] : most;
+        if (most > sum.m) sum = sum.at(most, c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum.add(SoftmaxSums::distance(v[j], sum.m, c));
+        if (a.top && __any(most > list.threshold)) list.take(v, most, id);
+    }
+    // The whole chunks, in pairs, with the next pair on its way. Past the end the last chunk is asked for again: a load under a
+    // condition would make the compiler wait for all of them. One copy of the work on a chunk: unrolled over a ring of four it
+    // was 45 KB of code, which a short call fetches as it goes.
+    template <typename LIST>
+    __device__ __forceinline__ void quickly(const LogprobArgs& a, SoftmaxSums& sum, LIST& list, float c) const {
+        const int lane = threadIdx.x & 63, final_chunk = part + (chunks - 1 - part) / parts * parts;
+        auto ask = [&](int chunk) { return load(chunk < final_chunk ? chunk : final_chunk); };
+        Raw first = ask(part), second = ask(part + parts);
+        float r = sum.m == -INFINITY ? 0.0f : -(sum.m * c);
+        for (int chunk = part; chunk <= final_chunk;) {
+            const Raw third = ask(chunk + 2 * parts), fourth = ask(chunk + 3 * parts);
+#pragma nounroll
+            for (int i = 0; i < 2 && chunk <= final_chunk; ++i) {
+                float v[8];
+                widen(first, v);
+                float most = v[0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) most = fmaxf(most, v[j]);
+                if (__any(most > sum.m)) {
+                    sum = sum.at(fmaxf(most, sum.m), c);
+                    r = sum.m == -INFINITY ? 0.0f : -(sum.m * c);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum.add(__builtin_fmaf(v[j], c, r));
+                if (a.top && __any(most > list.threshold)) list.take(v, most, head + chunk * kChunk + lane * 8);
+                first = second;
+                chunk += parts;
+            }
+            first = third;
+            second = fourth;
+        }
+    }
+
     template <typename LIST>
     __device__ __forceinline__ void walk(const LogprobArgs& a, SoftmaxSums& sum, LIST& list) const {
-        const int lane = threadIdx.x & 63;
+        const int lane = threadIdx.x & 63, done = head + chunks * kChunk;
         const float c = a.scale * 1.44269504088896341f;
-        // The hardware's maximum passes a signalling NaN on, quieted, and loses what it was compared with. A part whose sum turns
-        // out to be no number is therefore gone through once more for its list, with comparisons.
+        // A part that turns out to hold a NaN or values past what the quick form measures is gone through once more, slowly.
         for (bool careful = false;; careful = true) {
-            bool far = false;  // uniform
-            auto take = [&](const float (&v)[8], int id) {
-                float most = v[0];
-                if (careful) {
-                    most = -INFINITY;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) most = v[j] > most ? v[j] : most;
-                } else {
-#pragma unroll
-                    for (int j = 1; j < 8; ++j) most = fmaxf(most, v[j]);
-                    if (__any(most > sum.m)) {
-                        sum = sum.at(fmaxf(most, sum.m), c);
-                        far = __any(SoftmaxSums::far(sum.m));
-                    }
-                    if (far) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) sum.add(SoftmaxSums::distance(v[j], sum.m, c));
-                    } else {
-                        const float r = sum.m == -INFINITY ? 0.0f : -(sum.m * c);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) sum.add(__builtin_fmaf(v[j], c, r));
-                    }
+            for (int phase = 0; phase < 3; ++phase) {  // ahead of the boundary; whole chunks; what is left behind them
+                if (phase == 1 && !careful) {
+                    if (part < chunks) quickly(a, sum, list, c);
+                    continue;
                 }
-                if (a.top && __any(most > list.threshold)) list.take(v, id);
-            };
-            // Chunk -1 stands for the values ahead of the boundary, chunk `chunks` for those behind the last whole one. Two chunks
-            // are in flight ahead of the one that is worked on; past the end the last one is asked for again.
-            const int done = head + chunks * kChunk, end = chunks + (done < vocab && part == parts - 1);
-            Raw now{}, next{};
-            if (part < chunks) {
-                now = load(part);
-                next = load(part + parts < chunks ? part + parts : part);
+                const bool mine = phase == 0 ? part == 0 : phase == 1 || part == parts - 1;
+                const int stop = phase == 0 ? head : phase == 1 ? done : vocab;
+                for (int id = phase == 0 ? 0 : phase == 1 ? head + part * kChunk : done; mine && id < stop; id += parts * kChunk)
+                    slowly(a, sum, list, id + lane * 8, stop, c);
             }
-            for (int chunk = part == 0 && head ? -1 : part < chunks ? part : chunks; chunk < end;) {
-                float v[8];
-                int id;
-                if (unsigned(chunk) < unsigned(chunks)) {
-                    const Raw ahead = load(chunk + 2 * parts < chunks ? chunk + 2 * parts : chunk);
-                    widen(now, v);
-                    id = head + chunk * kChunk + lane * 8;
-                    now = next;
-                    next = ahead;
-                } else {
-                    id = (chunk < 0 ? 0 : done) + lane * 8;
-                    const int stop = chunk < 0 ? head : vocab;  // up to seven values, or under a chunk
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = id + j < stop ? value(id + j) : -INFINITY;
-                }
-                take(v, id);
-                // the last part comes by `chunks` whatever its own stride
-                chunk = chunk < 0 ? part : chunk < chunks && chunk + parts >= chunks && end > chunks ? chunks : chunk + parts;
-            }
-            if (careful || !a.top || !__any(sum.z != sum.z)) break;
-            list.key = list.floor = kNoKey;
+            if (careful || !__any(sum.z != sum.z || SoftmaxSums::far(sum.m))) break;
+            sum = SoftmaxSums{};
+            list.key = kNoKey;
             list.threshold = -INFINITY;
+            list.full = false;
         }
         sum.join_lanes(c);
     }
 };
+
+// The logit of a row's i-th given token, asked for ahead of the rest; `there` false for an id outside the vocabulary or past the last.
+struct GivenLogit {
+    float v;
+    bool there;
+};
+template <bool BF16>
+__device__ __forceinline__ GivenLogit given_logit(const LogprobArgs& a, long row, int i) {
+    const int id = i < a.n_given ? a.given[row * a.n_given + i] : -1;
+    GivenLogit g{0.0f, id >= 0 && id < a.vocab};
+    if (g.there) {
+        const long at = row * a.pitch + id;
+        if constexpr (BF16) g.v = __uint_as_float(uint32_t(static_cast<const uint16_t*>(a.logits)[at]) << 16);
+        else g.v = static_cast<const float*>(a.logits)[at];
+    }
+    return g;
+}
 
 // What a workgroup of THREADS makes of a row's joined sums and the parts' keys: N a thread, kNoKey for none. Every thread of
 // the workgroup comes here.
@@ -310,10 +382,9 @@ struct RowShared {
     uint64_t room[kRoom];
     uint32_t most[kGroups];
     int count, reached[64];
-    float share[16];  // of the waves' lists
 };
 template <bool BF16, int THREADS, int N>
-__device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const SoftmaxSums& sum, const uint64_t (&key)[N], RowShared& sh) {
+__device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const SoftmaxSums& sum, GivenLogit given, const uint64_t (&key)[N], RowShared& sh) {
     const int tid = threadIdx.x, lane = tid & 63;
     const float c = a.scale * 1.44269504088896341f, log_z = log2f(sum.z);
     constexpr float kLn2 = 0.69314718055994531f;
@@ -323,45 +394,72 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
     auto logprob = [&](float v) { return (v - sum.m) * a.scale - ln_z; };
     if (tid == 0 && a.entropy) a.entropy[row] = empty ? 0.0f : kLn2 * (log_z - sum.s / sum.z);
     for (int i = tid; i < a.n_given; i += THREADS) {
-        const int id = a.given[row * a.n_given + i];
-        float lp = __builtin_nanf("");
-        if (id >= 0 && id < a.vocab) {
-            const long at = row * a.pitch + id;
-            const float v = BF16 ? __uint_as_float(uint32_t(static_cast<const uint16_t*>(a.logits)[at]) << 16) : static_cast<const float*>(a.logits)[at];
-            lp = empty ? -INFINITY : logprob(v);
-        }
-        a.given_logprob[row * a.n_given + i] = lp;
+        if (i >= THREADS) given = given_logit<BF16>(a, row, i);
+        a.given_logprob[row * a.n_given + i] = !given.there ? __builtin_nanf("") : empty ? -INFINITY : logprob(given.v);
     }
     if (!a.top) return;
-    // The bound: values alone, from the maxima of kGroups groups of threads (all of a wave's where there are fewer threads).
-    constexpr int kLanes = THREADS > kGroups ? THREADS / kGroups : 1;  // of a group
+    constexpr bool kFew = N == 1 && THREADS / 64 * kTopMost <= kRoom;
+    if constexpr (kFew) {  // few enough to order as they are: a key's place is the number of larger ones
+        const int all = THREADS / 64 * a.top;
+        if (lane < a.top) sh.room[(tid >> 6) * a.top + lane] = key[0];
+        __syncthreads();
+        for (int i = tid; i < all; i += THREADS) {
+            const uint64_t k = sh.room[i];
+            int larger = 0, there = 0;
+#pragma unroll 8
+            for (int j = 0; j < all; ++j) {
+                const uint64_t o = sh.room[j];
+                larger += o > k;
+                there += o != kNoKey;
+            }
+            if (k != kNoKey && larger < a.top) {
+                a.top_ids[row * a.top + larger] = key_id(k);
+                a.top_logprob[row * a.top + larger] = logprob(key_value(k));
+            }
+            if (i >= there && i < a.top) {
+                a.top_ids[row * a.top + i] = -1;
+                a.top_logprob[row * a.top + i] = -INFINITY;
+            }
+        }
+    } else {
+    // The bound: values alone, from the maxima of kGroups groups of threads.
+    constexpr int kLanes = THREADS / kGroups;  // of a group
+    static_assert(THREADS % kGroups == 0 && kLanes <= 8, "the lanes' exchanges below");
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) most = uint32_t(key[i] >> 32) > most ? uint32_t(key[i] >> 32) : most;
-#pragma unroll
-    for (int d = 1; d < kLanes; d *= 2) {
-        const uint32_t o = __shfl_xor(most, d);
-        most = o > most ? o : most;
-    }
+    auto larger_of = [&](uint32_t o) { most = o > most ? o : most; };
+    if (kLanes > 1) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kQuadXor1, 0xf, 0xf, false)));
+    if (kLanes > 2) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kQuadXor2, 0xf, 0xf, false)));
+    if (kLanes > 4) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kHalfRowMirror, 0xf, 0xf, false)));
     if (tid % kLanes == 0) sh.most[tid / kLanes] = most;
-    if (THREADS < kGroups && tid < kGroups - THREADS) sh.most[THREADS + tid] = 0;
-    if (tid < 64) sh.reached[tid] = 0;
-    if (tid == 64 % THREADS) sh.count = 0;
+    if (tid >= THREADS - 64) sh.reached[lane] = 0;
+    if (tid == 64) sh.count = 0;
     __syncthreads();
     const uint32_t two[2] = {sh.most[lane], sh.most[64 + lane]};
-    uint64_t bound = uint64_t(reached_by<32>(two, a.top)) << 32;
+    uint64_t bound = uint64_t(reached_by<16>(two, a.top)) << 32;
     auto reach = [&](uint64_t k) {  // keys of this wave that reach k
         int n = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) n += int(__popcll(__ballot(key[i] != kNoKey && key[i] >= k)));
         return n;
     };
-    const int here = reach(bound);
-    int at = 0;
-    if (here && lane == 0) at = atomicAdd(&sh.count, here);  // a key's place in the result does not depend on which wave is first
-    at = __builtin_amdgcn_readfirstlane(at);
-    __syncthreads();
-    int count = sh.count;
+    auto gather = [&] {  // a key's place in the result does not depend on which wave is first here
+        const int here = reach(bound);
+        int at = 0;
+        if (here && lane == 0) at = atomicAdd(&sh.count, here);
+        at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool kept = key[i] != kNoKey && key[i] >= bound;
+            const uint64_t mask = __ballot(kept);
+            if (kept && at + lanes_below(mask) < kRoom) sh.room[at + lanes_below(mask)] = key[i];
+            at += int(__popcll(mask));
+        }
+        __syncthreads();
+        return sh.count;
+    };
+    int count = gather();
     if (count > kRoom) {  // many equal values, or lists that each hold all but one of the largest: the exact cut, bit by bit
         bound = 0;
         for (int bit = 63; bit >= 0; --bit) {
@@ -372,20 +470,8 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
         }
         if (tid == 0) sh.count = 0;
         __syncthreads();
-        const int exact = reach(bound);
-        if (exact && lane == 0) at = atomicAdd(&sh.count, exact);
-        at = __builtin_amdgcn_readfirstlane(at);
-        __syncthreads();
-        count = sh.count;  // `top`, or all there are
+        count = gather();  // `top`, or all there are
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const bool kept = key[i] != kNoKey && key[i] >= bound;
-        const uint64_t mask = __ballot(kept);
-        if (kept) sh.room[at + lanes_below(mask)] = key[i];
-        at += int(__popcll(mask));
-    }
-    __syncthreads();
     // a key's place is the number of larger ones
     for (int i = tid; i < count; i += THREADS) {
         const uint64_t k = sh.room[i];
@@ -403,74 +489,87 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
         a.top_ids[row * a.top + p] = -1;
         a.top_logprob[row * a.top + p] = -INFINITY;
     }
+    }
 }
 
 template <int WAVES>
-__device__ __forceinline__ TopList<WAVES> empty_list(float* shared, int top) {
+struct ListShared {
+    uint64_t batch[WAVES][64], turn[WAVES][64];
+    uint32_t shown[64];
+};
+template <int WAVES>
+__device__ __forceinline__ TopList<WAVES> empty_list(ListShared<WAVES>& sh, int top) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (WAVES > 1) {
-        if (threadIdx.x < WAVES) shared[threadIdx.x] = -INFINITY;
+    if (WAVES > 2) {
+        if (threadIdx.x < 64) sh.shown[threadIdx.x] = 0;
         __syncthreads();
     }
-    return TopList<WAVES>{shared, top, (top + WAVES - 1) / WAVES, wave};
+    return TopList<WAVES>{sh.shown, sh.batch[wave], sh.turn[wave], top, wave};
 }
 
-// A workgroup per row, a part for each of its WAVES waves.
+// A workgroup per row at a time, a part for each of its WAVES waves.
 template <bool BF16, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) logprob_row_kernel(const LogprobArgs a) {
     __shared__ float4 sums[WAVES];
     __shared__ RowShared shared;
+    __shared__ ListShared<WAVES> list_shared;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    SoftmaxSums sum;
-    TopList<WAVES> list = empty_list<WAVES>(shared.share, a.top);
-    RowPart<BF16>(a, blockIdx.x, wave, WAVES).walk(a, sum, list);
-    if (lane == 0) sums[wave] = make_float4(sum.m, sum.z, sum.s, 0.0f);
-    __syncthreads();
-    const float c = a.scale * 1.44269504088896341f;
-    sum = SoftmaxSums{};
-    if (lane < WAVES) sum = SoftmaxSums{sums[lane].x, sums[lane].y, sums[lane].z};
-    sum.join_lanes(c);
-    const uint64_t key[1] = {lane < a.top ? list.key : kNoKey};
-    write_row<BF16, 64 * WAVES>(a, blockIdx.x, sum, key, shared);
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const GivenLogit given = given_logit<BF16>(a, row, threadIdx.x);
+        SoftmaxSums sum;
+        TopList<WAVES> list = empty_list(list_shared, a.top);
+        RowPart<BF16>(a, row, wave, WAVES).walk(a, sum, list);
+        if (lane == 0) sums[wave] = make_float4(sum.m, sum.z, sum.s, 0.0f);
+        __syncthreads();
+        const float c = a.scale * 1.44269504088896341f;
+        sum = SoftmaxSums{};
+        if (lane < WAVES) sum = SoftmaxSums{sums[lane].x, sums[lane].y, sums[lane].z};
+        sum.join_lanes(c);
+        const uint64_t key[1] = {lane < a.top ? list.key : kNoKey};
+        write_row<BF16, 64 * WAVES>(a, row, sum, given, key, shared);
+        __syncthreads();
+    }
 }
 
 // A row over several workgroups: each wave leaves its part's sums and list in memory ...
 constexpr int kPartWaves = 4;
 template <bool BF16>
 __global__ void __launch_bounds__(64 * kPartWaves) logprob_part_kernel(const LogprobArgs a) {
-    __shared__ float shared[kPartWaves];
+    __shared__ ListShared<kPartWaves> shared;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long cell = long(blockIdx.x) * kPartWaves + wave;  // parts is a multiple of kPartWaves: a workgroup is of one row
     SoftmaxSums sum;
-    TopList<kPartWaves> list = empty_list<kPartWaves>(shared, a.top);
+    TopList<kPartWaves> list = empty_list(shared, a.top);
     RowPart<BF16>(a, cell / a.parts, int(cell % a.parts), a.parts).walk(a, sum, list);
     if (lane == 0) a.stats[cell] = make_float4(sum.m, sum.z, sum.s, 0.0f);
     if (lane < a.top) a.lists[cell * a.top + lane] = list.key;
 }
 
 // ... and a workgroup per row joins them, everything it reads asked for at once.
+constexpr int kJoinThreads = 512;
 template <bool BF16>
-__global__ void __launch_bounds__(1024) logprob_join_kernel(const LogprobArgs a) {
-    constexpr int N = kPartsMost * kTopMost / 1024;
+__global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(const LogprobArgs a) {
+    constexpr int N = kPartsMost * kTopMost / kJoinThreads;
     __shared__ RowShared shared;
     const int lane = threadIdx.x & 63;
     const long row = blockIdx.x;
     const float c = a.scale * 1.44269504088896341f;
     const float4* stats = a.stats + row * a.parts;
     const uint64_t* lists = a.lists + row * a.parts * a.top;
+    const GivenLogit given = given_logit<BF16>(a, row, threadIdx.x);
     float4 two[2];
     uint64_t key[N];
 #pragma unroll
     for (int i = 0; i < 2; ++i) two[i] = lane + 64 * i < a.parts ? stats[lane + 64 * i] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int at = int(threadIdx.x) + 1024 * i;
+        const int at = int(threadIdx.x) + kJoinThreads * i;
         key[i] = at < a.parts * a.top ? lists[at] : kNoKey;
     }
     SoftmaxSums sum{two[0].x, two[0].y, two[0].z};
     sum.join(SoftmaxSums{two[1].x, two[1].y, two[1].z}, c);
     sum.join_lanes(c);
-    write_row<BF16, 1024>(a, row, sum, key, shared);
+    write_row<BF16, kJoinThreads>(a, row, sum, given, key, shared);
 }
 
 }  // namespace m26g

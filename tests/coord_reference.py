@@ -73,8 +73,8 @@ def logprobs(logits, given, top, scale):
     """Per row: given log probabilities, entropy, top ids, their log probabilities, and a bound for each of the three numbers.
 
     A term exp(t - m) = 2^d is off by the roundings of scale * log2 e and its constant (relative 2 |t - m| U32), of d (|t - m| U32)
-    and two of the exponential; a lane adds at most vocab / 256 + 40 terms one after another (a row of more than two chunks of
-    512 values is at least four waves' work), and 20 joins follow, each of which rescales by a factor that is off like a term.
+    and two of the exponential; a lane adds at most vocab / 128 + 40 terms one after another (a row of more than two chunks of
+    512 values is at least two waves' work), and 20 joins follow, each of which rescales by a factor that is off like a term.
     The mean of |t - m| under the distribution is what the first part amounts to in Z. A log probability is (v - m) scale - ln Z:
     two roundings of the first part, two of the second, one of the difference."""
     rows, vocab = logits.shape
@@ -83,7 +83,7 @@ def logprobs(logits, given, top, scale):
     gl = np.full(given.shape, np.nan)
     ent, ids, lp = np.zeros(rows), np.full((rows, top), -1, np.int64), np.full((rows, top), -np.inf)
     tol_g, tol_h, tol_t = np.zeros(given.shape), np.zeros(rows), np.zeros((rows, top))
-    chain = vocab / 256 + 40 + 20
+    chain = vocab / 128 + 40 + 20
     for r in range(rows):
         row = t[r]
         numbers = np.where(np.isnan(row), -np.inf, row)

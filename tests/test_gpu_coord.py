@@ -400,7 +400,9 @@ def some_logits(rng, rows, vocab, half, masked=0.0):
 
 
 LENGTHS = [(1, 1), (1, 2), (4, 5), (2, 8), (3, 63), (2, 64), (5, 511), (4, 512), (3, 513), (2, 520), (3, 1031), (2, 4099), (40, 2050), (3, 50003), (1, 131072),
-           (2, 131075), (1100, 700)]
+           (2, 131075), (1100, 700),
+           # every form of the rule on sizes: rows over two, four and eight waves, over several workgroups, more rows than workgroups
+           (1600, 3000), (800, 9000), (600, 9000), (200, 4200), (100, 9000), (5000, 600), (4100, 40), (31, 1537)]
 
 
 @pytest.mark.parametrize("rows,vocab", LENGTHS)
