@@ -8,10 +8,10 @@
 // selection may add next to nothing to the common path.
 //
 // Selection. A wave keeps its part's largest values in order, one to a lane, and walks the part in ascending order, 512 values
-// at a time, with the top-th of them as a threshold. A value above it is put in its place with one comparison and one shift
-// over the lanes; an equal one need not be: `top` values of its size with lower ids are there. One comparison of each
-// lane's maximum, which the softmax needs anyway, and a scalar branch are the whole cost where nothing qualifies, which after i
-// chunks is all but top / i of them. The waves of a workgroup help each other: of the 64 values that they have on show, the
+// at a time, with the top-th of them as a threshold. Values above it wait in LDS until there are as many as the list is to
+// hold and are put in their places together; an equal one need not be: `top` values of its size with lower ids are there. One
+// comparison of each lane's maximum, which the softmax needs anyway, and a scalar branch are the whole cost where nothing
+// qualifies, which after i chunks is all but about top / i of them. The waves of a workgroup help each other: of the 64 values that they have on show, the
 // largest of each, the top-th largest is a bound that `top` values of the row reach. List entries are 64-bit keys, the value's bits in integer order above the
 // complemented id: a total order, so the result does not depend on who finds what when.
 //
@@ -147,24 +147,18 @@ struct TopList {
     int top, wave;
     uint64_t key = kNoKey;
     float threshold = -INFINITY;  // uniform: a value has to be above this one to matter
-    bool full = false;            // uniform: `top` keys are there
+    int waiting = 0;              // uniform: keys in `batch`
 
     __device__ __forceinline__ static uint64_t of_lane(uint64_t k, int lane) {
         return uint64_t(__builtin_amdgcn_readlane(uint32_t(k >> 32), lane)) << 32 | uint32_t(__builtin_amdgcn_readlane(uint32_t(k), lane));
     }
-    __device__ __forceinline__ void insert(uint64_t k) {  // k uniform and new
-        const bool above = key > k;
-        const int place = int(__popcll(__ballot(above)));  // the lanes above are the first ones
-        const uint64_t moved = uint64_t(__builtin_amdgcn_update_dpp(0u, uint32_t(key >> 32), 0x138, 0xf, 0xf, false)) << 32 |  // wave_shr:1
-                               uint32_t(__builtin_amdgcn_update_dpp(0u, uint32_t(key), 0x138, 0xf, 0xf, false));
-        key = above ? key : int(threadIdx.x & 63) == place ? k : moved;
-    }
-    // Puts up to 64 new keys, one to a lane, kNoKey for none, in their places: a key's place is the number of larger ones.
-    __device__ __forceinline__ void merge(uint64_t fresh, int n) {
+    // Puts what waits in its place: a key's place is the number of larger ones.
+    __device__ __forceinline__ void merge() {
         const int lane = threadIdx.x & 63;
+        wave_fence();
+        const uint64_t fresh = lane < waiting ? batch[lane] : kNoKey;
         int place = 0, moved = lane;
-        key = lane < top ? key : kNoKey;
-        for (int i = 0; i < n; ++i) {
+        for (int i = 0; i < waiting; ++i) {
             const uint64_t k = of_lane(fresh, i);
             const bool above = key > k;
             const int before = int(__popcll(__ballot(above)));  // places that the list's keys take ahead of this one
@@ -178,6 +172,7 @@ struct TopList {
         wave_fence();
         key = turn[lane];
         wave_fence();
+        waiting = 0;
     }
     // What the values on show vouch for: `top` values of the row reach it, at any ids, so equal ones still count.
     __device__ __forceinline__ void common() {
@@ -185,59 +180,38 @@ struct TopList {
         const uint32_t bound = reached_by<16>(v, top);
         if (bound > order_bits(-INFINITY)) threshold = fmaxf(threshold, just_below(order_value(bound)));
     }
-    // The slow path of a chunk. Element j of the lane has id `id` + j; `most` is the lane's maximum.
-    __device__ __forceinline__ void take(const float (&v)[8], float most, int id) {
-        const int lane = threadIdx.x & 63;
-        if constexpr (WAVES > 2) {  // two waves gain less than the look costs
-            common();
-            if (!__any(most > threshold)) return;
-        }
-        if (!full) {
-            // Not `top` values yet: what `top` of the lanes' maxima reach, as many values of this chunk do.
+    // The slow path of a chunk. Element j of the lane has id `id` + j. What is above the threshold waits, and is put in its place
+    // when as much waits as the list is to hold: a place costs 50 cycles then, in a list of its own 300.
+    __device__ __forceinline__ void take(const float (&v)[8], int id) {
+        if (threshold == -INFINITY) {
+            // Nothing known yet: what `top` of the lanes' maxima reach, as many values of this chunk do.
             float largest = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) largest = v[j] > largest ? v[j] : largest;  // a NaN takes no part
             const uint32_t mine[1] = {order_bits(largest)};
             const uint32_t bound = reached_by<16>(mine, top);
-            if (bound > order_bits(-INFINITY)) threshold = fmaxf(threshold, just_below(order_value(bound)));
+            if (bound > order_bits(-INFINITY)) threshold = just_below(order_value(bound));
         }
-        // Within the chunk ids are not met in order, so all values above the threshold join, and their keys find the order.
-        int n = 0;
+        // Within the chunk ids are not met in order, so the threshold stays as it is until its end.
 #pragma unroll
-        for (int j = 0; j < 8; ++j) n += int(__popcll(__ballot(v[j] > threshold)));
-        if (n <= 3) {  // one at a time
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                for (uint64_t mask = __ballot(v[j] > threshold); mask; mask &= mask - 1) {
-                    const int from = __ffsll(static_cast<unsigned long long>(mask)) - 1;
-                    const float one = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[j]), from));
-                    insert(list_key(one, __builtin_amdgcn_readlane(id, from) + j));
-                }
-        } else {  // up to 64 at a time
-            n = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool wanted = v[j] > threshold;
-                const uint64_t mask = __ballot(wanted);
-                if (n + int(__popcll(mask)) > 64) {
-                    wave_fence();
-                    merge(lane < n ? batch[lane] : kNoKey, n);
-                    n = 0;
-                }
-                if (wanted) batch[n + lanes_below(mask)] = list_key(v[j], id + j);
-                n += int(__popcll(mask));
-            }
-            wave_fence();
-            merge(lane < n ? batch[lane] : kNoKey, n);
+        for (int j = 0; j < 8; ++j) {
+            const bool wanted = v[j] > threshold;
+            const uint64_t mask = __ballot(wanted);
+            if (!mask) continue;
+            const int n = int(__popcll(mask));
+            if (waiting + n > 64) merge();
+            if (wanted) batch[waiting + lanes_below(mask)] = list_key(v[j], id + j);
+            waiting += n;
         }
+        if (waiting < (top < 8 ? 8 : top)) return;
+        const int lane = threadIdx.x & 63;
+        merge();
         const uint32_t last = __builtin_amdgcn_readlane(uint32_t(key >> 32), top - 1);
-        if (last) {
-            full = true;
-            threshold = fmaxf(threshold, order_value(last));
-        }
-        if constexpr (WAVES > 2) {
+        if (last) threshold = fmaxf(threshold, order_value(last));
+        if constexpr (WAVES > 2) {  // two waves gain less than it costs
             constexpr int kShow = 64 / WAVES;
             if (lane < kShow && lane < top) __hip_atomic_store(&shown[wave * kShow + lane], uint32_t(key >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            common();
         }
     }
 };
@@ -297,7 +271,7 @@ struct RowPart {
         if (most > sum.m) sum = sum.at(most, c);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum.add(SoftmaxSums::distance(v[j], sum.m, c));
-        if (a.top && __any(most > list.threshold)) list.take(v, most, id);
+        if (a.top && __any(most > list.threshold)) list.take(v, id);
     }
     // The whole chunks, in pairs, with the next pair on its way. Past the end the last chunk is asked for again: a load under a
     // condition would make the compiler wait for all of them. One copy of the work on a chunk: unrolled over a ring of four it
@@ -323,7 +297,7 @@ struct RowPart {
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum.add(__builtin_fmaf(v[j], c, r));
-                if (a.top && __any(most > list.threshold)) list.take(v, most, head + chunk * kChunk + lane * 8);
+                if (a.top && __any(most > list.threshold)) list.take(v, head + chunk * kChunk + lane * 8);
                 first = second;
                 chunk += parts;
             }
@@ -352,9 +326,10 @@ struct RowPart {
             sum = SoftmaxSums{};
             list.key = kNoKey;
             list.threshold = -INFINITY;
-            list.full = false;
+            list.waiting = 0;
         }
         sum.join_lanes(c);
+        if (list.waiting) list.merge();
     }
 };
 
