@@ -17,8 +17,9 @@ bool on(const void* p, uintptr_t boundary) { return address(p) % boundary == 0; 
 
 // ---- block join
 template <int T, int NG>
-void launch_join(const JoinArgs& a, bool vec, unsigned grid, hipStream_t st) {
-    if (vec) block_join_kernel<T, NG, true><<<grid, T, 0, st>>>(a);
+void launch_join(const JoinArgs& a, hipStream_t st) {
+    const unsigned grid = unsigned(a.rows < 65536 ? a.rows : 65536);
+    if (a.cols % 8) block_join_kernel<T, NG, true><<<grid, T, 0, st>>>(a);
     else block_join_kernel<T, NG, false><<<grid, T, 0, st>>>(a);
 }
 
@@ -50,8 +51,8 @@ int launch_logprobs(const LogprobArgs& a, hipStream_t st) {
         logprob_join_kernel<BF16><<<unsigned(a.rows), kJoinThreads, 0, st>>>(a);
         return launched();
     }
-    // Waves to a row: as few as fill the chip, since each finds its own largest values first (2048 rows x 131072: two waves
-    // 103 us, four 118, eight 133; 1024 x 50003: four 49, two 63).
+    // Waves to a row: as few as fill the chip, since each finds its own largest values first (2000 x 20000, top 30: two waves 52
+    // us, four 60, eight 97; 1024 x 50003, top 20: four 43, two 52, eight 49; 600 x 100000, top 5: eight 37, four 40).
     const int chunks = a.vocab / kChunk;
     if (chunks <= 2 && (a.rows >= 768 || chunks == 0)) return launch_rows<BF16, 1>(a, st);
     if (a.rows >= 1536) return launch_rows<BF16, 2>(a, st);
@@ -169,18 +170,9 @@ int m26c_block_join(const m26c_join* plan, long rows, const float* h, const uint
         (norm && p.norm_pitch < p.cols))
         return 1;
     if (payload && (p.cols % 32 || p.payload_pitch < size_t(p.cols) || p.scales_pitch < size_t(p.cols / 32))) return 1;
-    bool vec = p.cols % 8 == 0 && p.plane_pitch % 8 == 0 && p.h_pitch % 4 == 0 && on(h, 16) && on(h_out, 16) && on(norm, 16) &&
-               (!norm || p.norm_pitch % 8 == 0) && on(p.pre_weight, 16) && on(p.post_weight, 16) && on(payload, 8) &&
-               (!payload || p.payload_pitch % 8 == 0);
-    if (!on(h, 4) || !on(h_out, 4) || !on(norm, 2) || !on(p.pre_weight, 4) || !on(p.post_weight, 4)) return 1;
-    for (int i = 0; i < p.planes; ++i) {
+    if (!on(h, 4) || !on(h_out, 4) || !on(norm, 2) || !on(p.pre_weight, 4) || !on(p.post_weight, 4) || (p.gate_cols && !on(gate, 4))) return 1;
+    for (int i = 0; i < p.planes; ++i)
         if (!planes[i] || !on(planes[i], 2)) return 1;
-        vec = vec && on(planes[i], 16);
-    }
-    if (p.gate_cols) {
-        if (!on(gate, 4)) return 1;
-        if (p.gate_cols > 1) vec = vec && on(gate, 16) && p.gate_pitch % 4 == 0;
-    }
     JoinArgs a{};
     for (int i = 0; i < p.planes; ++i) a.plane[i] = planes[i];
     a.h = h; a.gate = gate; a.pre_w = p.pre_weight; a.post_w = p.post_weight;
@@ -188,12 +180,18 @@ int m26c_block_join(const m26c_join* plan, long rows, const float* h, const uint
     a.rows = rows; a.plane_pitch = p.plane_pitch; a.h_pitch = p.h_pitch; a.norm_pitch = p.norm_pitch; a.gate_pitch = p.gate_pitch;
     a.payload_pitch = p.payload_pitch; a.scales_pitch = p.scales_pitch;
     a.cols = p.cols; a.planes = p.planes; a.gate_cols = p.gate_cols; a.scale = p.scale; a.eps = p.eps;
-    const unsigned grid = unsigned(rows < 65536 ? rows : 65536);
     hipStream_t st = hipStream_t(stream);
-    if (p.cols <= 2048) launch_join<256, 1>(a, vec, grid, st);
-    else if (p.cols <= 4096) launch_join<256, 2>(a, vec, grid, st);
-    else if (p.cols <= 8192) launch_join<512, 2>(a, vec, grid, st);
-    else launch_join<1024, 2>(a, vec, grid, st);
+    if (rows < 512) {  // few rows: as many threads to a row as it has groups
+        if (p.cols <= 2048) launch_join<256, 1>(a, st);
+        else if (p.cols <= 4096) launch_join<512, 1>(a, st);
+        else if (p.cols <= 8192) launch_join<1024, 1>(a, st);
+        else launch_join<1024, 2>(a, st);
+    } else {
+        if (p.cols <= 2048) launch_join<256, 1>(a, st);
+        else if (p.cols <= 4096) launch_join<256, 2>(a, st);
+        else if (p.cols <= 8192) launch_join<512, 2>(a, st);
+        else launch_join<1024, 2>(a, st);
+    }
     return launched();
 }
 

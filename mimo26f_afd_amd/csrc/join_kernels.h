@@ -51,12 +51,24 @@ __device__ __forceinline__ uint32_t q0_byte_of_block(uint32_t most, float amax_o
 }
 __device__ __forceinline__ float q0_inverse(uint32_t s) { return __uint_as_float(s == 254u ? 0x00400000u : (254u - s) << 23); }
 
-// A workgroup per row at a time. VEC: a thread holds NG groups of eight neighbouring values, T groups apart (16-byte
-// accesses); otherwise 8 * NG single values, T apart.
-template <int T, int NG, bool VEC>
+// Sixteen bytes at any alignment of the element: the memory path takes them as they come, an odd row costs it a line more.
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef v4f v4f_any __attribute__((aligned(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef v4u v4u_any __attribute__((aligned(2)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+typedef v2u v2u_any __attribute__((aligned(1)));
+
+// A workgroup of T threads per row at a time; a thread holds NG groups of eight neighbouring values, T groups apart. With RAGGED the
+// row's last group is the last eight values, of which the first ones belong to the group before it: they count as zero and
+// are not written. (Loads value by value under a condition wait for one another: 1021 rows x 2047, two planes 11.0 us
+// against 9.2.) Rows of
+// under eight values are loaded value by value.
+template <int T, int NG, bool RAGGED>
 __global__ void __launch_bounds__(T) block_join_kernel(const JoinArgs a) {
     constexpr int WAVES = T / 64, N = 8 * NG;
-    __shared__ float parts[2][WAVES];  // the two sums take turns, so a row's second barrier also guards its first sum's slots
+    constexpr int LIVE = T == 1024 && NG == 2 && RAGGED ? 1 : 4;  // planes on their way together, as the 128 registers of a lane allow
+    __shared__ float parts[2][WAVES];  // the sums take turns: who writes a slot again has passed the barrier behind its last readers
     const int tid = threadIdx.x, wave = tid >> 6;
     int turn = 0;
     auto row_sum = [&](float v) {
@@ -69,38 +81,61 @@ __global__ void __launch_bounds__(T) block_join_kernel(const JoinArgs a) {
         turn ^= 1;
         return s;
     };
-    // value i of this thread is column column(i); in_row(i) for whole groups of eight when VEC
-    auto column = [&](int i) { return VEC ? (tid + T * (i >> 3)) * 8 + (i & 7) : tid + T * i; };
+    // Of group j: whether it has values in the row, the column of its first one, and how many of them are not its own.
+    auto there = [&](int j) { return (tid + T * j) * 8 < a.cols; };
+    auto short_by = [&](int j) { return RAGGED && there(j) && (tid + T * j) * 8 + 8 > a.cols ? (tid + T * j) * 8 + 8 - a.cols : 0; };
+    auto column = [&](int j) { return (tid + T * j) * 8 - (RAGGED && a.cols >= 8 ? short_by(j) : 0); };
+    auto owned = [&](int j, int i) { return !RAGGED || (a.cols >= 8 ? i >= short_by(j) : i < a.cols); };
+    const bool tiny = RAGGED && a.cols < 8;
     auto floats = [&](const float* p, float (&v)[N]) {  // one row of floats
-        if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                const int c = column(8 * j);
-                float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-                if (c < a.cols) { lo = *reinterpret_cast<const float4*>(p + c); hi = *reinterpret_cast<const float4*>(p + c + 4); }
-                v[8 * j] = lo.x; v[8 * j + 1] = lo.y; v[8 * j + 2] = lo.z; v[8 * j + 3] = lo.w;
-                v[8 * j + 4] = hi.x; v[8 * j + 5] = hi.y; v[8 * j + 6] = hi.z; v[8 * j + 7] = hi.w;
+        for (int j = 0; j < NG; ++j) {
+            v4f lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+            if (there(j)) {
+                if (!tiny) {
+                    lo = *reinterpret_cast<const v4f_any*>(p + column(j));
+                    hi = *reinterpret_cast<const v4f_any*>(p + column(j) + 4);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i < a.cols) lo[i] = p[i];
+                        if (4 + i < a.cols) hi[i] = p[4 + i];
+                    }
+                }
             }
-        } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = column(i) < a.cols ? p[column(i)] : 0.0f;
+            for (int i = 0; i < 4; ++i) { v[8 * j + i] = lo[i]; v[8 * j + 4 + i] = hi[i]; }
         }
     };
-    auto halves = [&](const uint16_t* p, float (&v)[N]) {  // one row of BF16 values
-        if constexpr (VEC) {
+    auto halves = [&](const uint16_t* p, v4u (&v)[NG]) {  // one row of BF16 values, as they lie
 #pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                const int c = column(8 * j);
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (c < a.cols) w = *reinterpret_cast<const uint4*>(p + c);
-                const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+        for (int j = 0; j < NG; ++j) {
+            v[j] = v4u{0, 0, 0, 0};
+            if (!there(j)) continue;
+            if (!tiny) {
+                v[j] = *reinterpret_cast<const v4u_any*>(p + column(j));
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) { v[8 * j + 2 * i] = __uint_as_float(d[i] << 16); v[8 * j + 2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u); }
+                for (int i = 0; i < 8; ++i)
+                    if (i < a.cols) v[j][i / 2] |= uint32_t(p[i]) << (16 * (i & 1));
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] = column(i) < a.cols ? __uint_as_float(uint32_t(p[column(i)]) << 16) : 0.0f;
         }
+    };
+    auto own = [&](float (&v)[N]) {
+        if constexpr (RAGGED)
+#pragma unroll
+            for (int j = 0; j < NG; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[8 * j + i] = owned(j, i) ? v[8 * j + i] : 0.0f;
+    };
+    auto add = [&](float (&z)[N], const v4u (&v)[NG]) {
+#pragma unroll
+        for (int j = 0; j < NG; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                z[8 * j + 2 * i] += __uint_as_float(v[j][i] << 16);
+                z[8 * j + 2 * i + 1] += __uint_as_float(v[j][i] & 0xffff0000u);
+            }
     };
     auto squares = [&](const float (&v)[N]) {
         float s = 0.0f;
@@ -111,15 +146,27 @@ __global__ void __launch_bounds__(T) block_join_kernel(const JoinArgs a) {
     const float inv_cols = 1.0f / float(a.cols);
     for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         float z[N], h[N], t[N];
-        halves(a.plane[0] + r * a.plane_pitch, z);
-        floats(a.h + r * a.h_pitch, h);
-        for (int p = 1; p < a.planes; ++p) {
-            halves(a.plane[p] + r * a.plane_pitch, t);
+        v4u plane[LIVE][NG];
+        halves(a.plane[0] + r * a.plane_pitch, plane[0]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) z[i] += t[i];
-        }
+        for (int p = 1; p < LIVE; ++p)
+            if (p < a.planes) halves(a.plane[p] + r * a.plane_pitch, plane[p]);
+        floats(a.h + r * a.h_pitch, h);
+        if (a.post_w) floats(a.post_w, t);
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = 0.0f;
+        add(z, plane[0]);
+#pragma unroll
+        for (int p = 1; p < LIVE; ++p)
+            if (p < a.planes) add(z, plane[p]);
+#pragma unroll
+        for (int p = LIVE; p < 4; ++p)
+            if (p < a.planes) {
+                halves(a.plane[p] + r * a.plane_pitch, plane[0]);
+                add(z, plane[0]);
+            }
+        own(z);
         if (a.post_w) {
-            floats(a.post_w, t);
             const float k = 1.0f / sqrtf(row_sum(squares(z)) * inv_cols + a.eps);
 #pragma unroll
             for (int i = 0; i < N; ++i) z[i] = z[i] * k * t[i];
@@ -133,20 +180,21 @@ __global__ void __launch_bounds__(T) block_join_kernel(const JoinArgs a) {
 #pragma unroll
             for (int i = 0; i < N; ++i) h[i] += g * z[i];
         }
+        own(h);  // behind the gate: an infinite one makes NaN of a zero
         if (a.h_out) {
             float* o = a.h_out + r * a.h_pitch;
-            if constexpr (VEC) {
 #pragma unroll
-                for (int j = 0; j < NG; ++j) {
-                    const int c = column(8 * j);
-                    if (c >= a.cols) continue;
-                    *reinterpret_cast<float4*>(o + c) = make_float4(h[8 * j], h[8 * j + 1], h[8 * j + 2], h[8 * j + 3]);
-                    *reinterpret_cast<float4*>(o + c + 4) = make_float4(h[8 * j + 4], h[8 * j + 5], h[8 * j + 6], h[8 * j + 7]);
+            for (int j = 0; j < NG; ++j) {
+                const int c = column(j);
+                if (!there(j)) continue;
+                if (!RAGGED || short_by(j) == 0) {
+                    *reinterpret_cast<v4f_any*>(o + c) = v4f{h[8 * j], h[8 * j + 1], h[8 * j + 2], h[8 * j + 3]};
+                    *reinterpret_cast<v4f_any*>(o + c + 4) = v4f{h[8 * j + 4], h[8 * j + 5], h[8 * j + 6], h[8 * j + 7]};
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (owned(j, i)) o[c + i] = h[8 * j + i];
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (column(i) < a.cols) o[column(i)] = h[i];
             }
         }
         if (!a.norm && !a.payload) continue;  // the same for every thread
@@ -156,62 +204,46 @@ __global__ void __launch_bounds__(T) block_join_kernel(const JoinArgs a) {
         for (int i = 0; i < N; ++i) h[i] = h[i] * k * t[i];
         if (a.norm) {
             uint16_t* o = a.norm + r * a.norm_pitch;
-            if constexpr (VEC) {
 #pragma unroll
-                for (int j = 0; j < NG; ++j) {
-                    const int c = column(8 * j);
-                    if (c >= a.cols) continue;
-                    const float* v = h + 8 * j;
-                    *reinterpret_cast<uint4*>(o + c) = make_uint4(bf16_rne_nan(v[0]) | bf16_rne_nan(v[1]) << 16, bf16_rne_nan(v[2]) | bf16_rne_nan(v[3]) << 16,
-                                                                  bf16_rne_nan(v[4]) | bf16_rne_nan(v[5]) << 16, bf16_rne_nan(v[6]) | bf16_rne_nan(v[7]) << 16);
+            for (int j = 0; j < NG; ++j) {
+                const int c = column(j);
+                if (!there(j)) continue;
+                if (!RAGGED || short_by(j) == 0) {
+                    v4u w;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = bf16_rne_nan(h[8 * j + 2 * i]) | bf16_rne_nan(h[8 * j + 2 * i + 1]) << 16;
+                    *reinterpret_cast<v4u_any*>(o + c) = w;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (owned(j, i)) o[c + i] = uint16_t(bf16_rne_nan(h[8 * j + i]));
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (column(i) < a.cols) o[column(i)] = uint16_t(bf16_rne_nan(h[i]));
             }
         }
         if (!a.payload) continue;
-        // Wire rows. A block of 32 values is four neighbouring lanes when VEC, half a wave otherwise; cols is a multiple
-        // of 32 here, so a block is in the row as a whole or not at all.
+        // Wire rows: a block of 32 values is four neighbouring lanes; cols is a multiple of 32 here, so a block is in the row as
+        // a whole or not at all.
         auto numbers = [](float f) { return f != f ? 0.0f : fabsf(f); };
-        if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                const float* v = h + 8 * j;
-                const int c = column(8 * j);
-                uint32_t most = 0;
+        for (int j = 0; j < NG; ++j) {
+            const float* v = h + 8 * j;
+            const int c = column(j);
+            uint32_t most = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) { const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu; most = m > most ? m : most; }
-                most = max_bits_over_four(most);
-                float amax = 0.0f;
-                if (most >= 0x7f800000u) {
+            for (int i = 0; i < 8; ++i) { const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu; most = m > most ? m : most; }
+            most = max_bits_over_four(most);
+            float amax = 0.0f;
+            if (most >= 0x7f800000u) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, numbers(v[i]));
-                    amax = __uint_as_float(max_bits_over_four(__float_as_uint(amax)));
-                }
-                if (c >= a.cols) continue;
-                const uint32_t s = q0_byte_of_block(most, amax);
-                const float inv = q0_inverse(s);
-                *reinterpret_cast<uint2*>(a.payload + r * a.payload_pitch + c) =
-                    make_uint2(e4m3_half_up4(make_float4(v[0], v[1], v[2], v[3]), inv), e4m3_half_up4(make_float4(v[4], v[5], v[6], v[7]), inv));
-                if ((tid & 3) == 0) a.scales[r * a.scales_pitch + c / 32] = uint8_t(s);
+                for (int i = 0; i < 8; ++i) amax = fmaxf(amax, numbers(v[i]));
+                amax = __uint_as_float(max_bits_over_four(__float_as_uint(amax)));
             }
-        } else {
-            for (int i = 0; i < N; ++i) {
-                uint32_t most = __float_as_uint(h[i]) & 0x7fffffffu;
-                float amax = numbers(h[i]);
-#pragma unroll
-                for (int d = 1; d < 32; d *= 2) {
-                    const uint32_t m = __shfl_xor(most, d);
-                    most = m > most ? m : most;
-                    amax = fmaxf(amax, __shfl_xor(amax, d));
-                }
-                if (column(i) >= a.cols) continue;
-                const uint32_t s = q0_byte_of_block(most, amax);
-                a.payload[r * a.payload_pitch + column(i)] = uint8_t(e4m3_half_up(h[i], q0_inverse(s)));
-                if ((tid & 31) == 0) a.scales[r * a.scales_pitch + column(i) / 32] = uint8_t(s);
-            }
+            if (!there(j)) continue;
+            const uint32_t s = q0_byte_of_block(most, amax);
+            const float inv = q0_inverse(s);
+            *reinterpret_cast<v2u_any*>(a.payload + r * a.payload_pitch + c) =
+                v2u{e4m3_half_up4(make_float4(v[0], v[1], v[2], v[3]), inv), e4m3_half_up4(make_float4(v[4], v[5], v[6], v[7]), inv)};
+            if ((tid & 3) == 0) a.scales[r * a.scales_pitch + c / 32] = uint8_t(s);
         }
     }
 }

@@ -174,6 +174,28 @@ def test_join_keeps_a_bad_row_to_itself_and_a_zero_row_at_zero():
     assert (got["h"][3] == 0).all() and (R.widen(got["norm"][3]) == 0).all() and (R.wire_values(got["payload"][3], got["scales"][3]) == 0).all()
 
 
+@pytest.mark.parametrize("cols", [9, 2047, 4097, 12001])
+def test_join_infinite_gate_stays_at_its_column_on_odd_rows(cols):
+    """A column next to the row's end: an infinite h' there makes the norm's factor zero, the other columns' n zero and its own NaN."""
+    h, planes, pre, pw, gate = join_inputs(3, cols, 2, True, "column", cols)
+    at = cols - cols % 8 - 1
+    gate[0, at] = np.inf
+    got = run_join(h, planes, pre, pw, gate, 1.0, 1e-5, "column", wire=False)
+    rest = np.arange(cols) != at
+    assert np.isinf(got["h"][:, at]).all() and np.isfinite(got["h"][:, rest]).all()
+    n = R.widen(got["norm"])
+    assert np.isnan(n[:, at]).all() and (n[:, rest] == 0).all()
+
+
+@pytest.mark.parametrize("rows,cols,planes,post,gate", [(600, 2050, 4, True, "full"), (515, 5001, 3, True, "row"), (513, 9999, 4, False, "column"),
+                                                        (520, 4160, 2, True, "full")])
+def test_join_many_longer_rows(rows, cols, planes, post, gate):
+    args = join_inputs(rows, cols, planes, post, gate, cols)
+    wire = cols % 32 == 0
+    check_join(run_join(*args, 0.5, 1e-5, gate, wire=wire), *args, 0.5, 1e-5)
+    check_join(run_join(*args, 0.5, 1e-5, gate, wire=wire, in_place=True, shift=3), *args, 0.5, 1e-5)
+
+
 def test_join_many_rows_walk_the_grid():
     """More rows than workgroups in a launch; small rows keep it quick."""
     args = join_inputs(70001, 32, 1, True, "row", 5)
