@@ -41,7 +41,7 @@ class Join:
         self._plan = _JoinPlan(cols, planes, plane_pitch or cols, h_pitch or cols, norm_pitch or cols, pre_weight, post_weight, gate_cols,
                                gate_pitch, scale, eps, payload_pitch or cols, scales_pitch or cols // 32)
         self._ref = C.byref(self._plan)
-        self._planes = planes
+        self._planes, self._rest = planes, (None,) * (4 - planes)
         self._call = load().m26c_block_join
 
     def __call__(self, rows: int, h: int, planes, h_out: int | None, norm: int | None = None, gate: int | None = None,
@@ -50,8 +50,9 @@ class Join:
         be None, as long as one is not."""
         if len(planes) != self._planes:
             raise CoordError(1, f"block join of {self._planes} planes called with {len(planes)}")
-        p = (*planes, None, None, None, None)
-        _ck(self._call(self._ref, rows, h, p[0], p[1], p[2], p[3], gate, h_out, norm, payload, scales, stream), "block join")
+        rc = self._call(self._ref, rows, h, *planes, *self._rest, gate, h_out, norm, payload, scales, stream)
+        if rc:
+            raise CoordError(rc, "block join")
 
 
 class Weights4:

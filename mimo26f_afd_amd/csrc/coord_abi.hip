@@ -24,15 +24,28 @@ void launch_join(const JoinArgs& a, hipStream_t st) {
 }
 
 // ---- log probabilities
-// Parts of a row over several workgroups, about 4096 waves over all rows and two chunks each at least; 0 where that
-// leaves a row fewer than eight and a workgroup takes whole rows (us a pass: 1 row x 131072 logits 13.2 against 30.6 with a
-// workgroup of eight waves, 37 x 50003 14.6 against 18.4, 300 x 131072 44 against 50).
-int parts_of(int rows, int vocab) {
+// How a call is cut, by rows and vocabulary alone (us a pass; walking / short parts):
+//  * up to two waves' registers hold a row: a workgroup per row, short parts (16384 x 1000 BF16, top 5: 39 / 26)
+//  * up to eight, as long as the chip holds all rows at once (512 x 8000, top 5: 11.8 / 9.6; 2048 x 8000 18.1 / 30.2 the other way)
+//  * few rows: over several workgroups in short parts of two chunks, of four where 128 parts would not reach (1 row x 131072
+//    FP32, top 20: 13.9 / 9.8; 128 x 50003 BF16, top 5: 17.4 / 14.9; 600 x 20000, top 5: 17.5 / 20.9 the other way)
+//  * otherwise waves walk: over parts, about 4096 waves over all rows and two chunks each at least, or over whole rows where
+//    that leaves a row fewer than eight parts (300 x 131072: 44 against 50).
+struct LogprobCut {
+    int parts;   // over several workgroups, 0: a workgroup takes whole rows
+    int chunks;  // of a short part, 0: waves walk
+};
+LogprobCut cut_of(int rows, int vocab) {
+    const int waves = (vocab + 2 * kChunk - 1) / (2 * kChunk);
+    if (waves <= 2 || (waves <= 8 && long(waves) * rows <= 4096)) return {0, 2};
+    const int chunks = vocab <= 2 * kChunk * kPartsMost ? 2 : 4;
+    const long parts4 = (long(vocab) + chunks * kChunk * kPartWaves - 1) / (chunks * kChunk * kPartWaves), short_parts = parts4 * kPartWaves;
+    if (short_parts <= kPartsMost && short_parts * rows <= 8192) return {int(short_parts), chunks};
     int parts = vocab / kChunk / 2;
     parts = parts < 4096 / rows ? parts : 4096 / rows;
     parts = parts < kPartsMost ? parts : kPartsMost;
     parts = parts / kPartWaves * kPartWaves;
-    return parts < 8 ? 0 : parts;
+    return {parts < 8 ? 0 : parts, 0};
 }
 size_t stats_bytes(int rows, int parts) { return size_t(rows) * parts * sizeof(float4); }
 
@@ -43,20 +56,35 @@ int launch_rows(const LogprobArgs& a, hipStream_t st) {
     return launched();
 }
 
+template <bool BF16, int WAVES>
+int launch_short_rows(const LogprobArgs& a, hipStream_t st) {
+    const int wide = a.rows < 16384 ? a.rows : 16384;
+    logprob_short_row_kernel<BF16, WAVES, 2><<<unsigned(wide), 64 * WAVES, 0, st>>>(a);
+    return launched();
+}
+
 template <bool BF16>
-int launch_logprobs(const LogprobArgs& a, hipStream_t st) {
+int launch_logprobs(const LogprobArgs& a, int short_chunks, hipStream_t st) {
     if (a.parts) {
-        logprob_part_kernel<BF16><<<unsigned(a.rows) * unsigned(a.parts / kPartWaves), 64 * kPartWaves, 0, st>>>(a);
+        const unsigned grid = unsigned(a.rows) * unsigned(a.parts / kPartWaves);
+        if (short_chunks == 2) logprob_short_part_kernel<BF16, 2><<<grid, 64 * kPartWaves, 0, st>>>(a);
+        else if (short_chunks == 4) logprob_short_part_kernel<BF16, 4><<<grid, 64 * kPartWaves, 0, st>>>(a);
+        else logprob_part_kernel<BF16><<<grid, 64 * kPartWaves, 0, st>>>(a);
         if (int rc = launched()) return rc;
         logprob_join_kernel<BF16><<<unsigned(a.rows), kJoinThreads, 0, st>>>(a);
         return launched();
     }
+    if (short_chunks) {
+        const int waves = (a.vocab + 2 * kChunk - 1) / (2 * kChunk);
+        if (waves == 1) return launch_short_rows<BF16, 1>(a, st);
+        if (waves == 2) return launch_short_rows<BF16, 2>(a, st);
+        if (waves <= 4) return launch_short_rows<BF16, 4>(a, st);
+        return launch_short_rows<BF16, 8>(a, st);
+    }
     // Waves to a row: as few as fill the chip, since each finds its own largest values first (2000 x 20000, top 30: two waves 52
     // us, four 60, eight 97; 1024 x 50003, top 20: four 43, two 52, eight 49; 600 x 100000, top 5: eight 37, four 40).
-    const int chunks = a.vocab / kChunk;
-    if (chunks <= 2 && (a.rows >= 768 || chunks == 0)) return launch_rows<BF16, 1>(a, st);
     if (a.rows >= 1536) return launch_rows<BF16, 2>(a, st);
-    if (a.rows >= 768 || chunks < 16) return launch_rows<BF16, 4>(a, st);
+    if (a.rows >= 768 || a.vocab < 16 * kChunk) return launch_rows<BF16, 4>(a, st);
     return launch_rows<BF16, 8>(a, st);
 }
 
@@ -252,22 +280,28 @@ int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_
     return w4_run(w, a, true, stream);
 }
 
+constexpr int kVocabMost = 1 << 30;           // ids past a row's end, up to a chunk of every part, still fit
+constexpr float kScaleMost = float(1 << 20);  // a scaled logit that is measured from a rounded maximum stays finite
+
 size_t m26c_token_logprobs_workspace(int rows, int vocab, int top) {
-    if (rows <= 0 || vocab <= 0 || top < 0 || top > kTopMost) return 0;
-    const int parts = parts_of(rows, vocab);
+    if (rows <= 0 || vocab <= 0 || vocab > kVocabMost || top < 0 || top > kTopMost) return 0;
+    const int parts = cut_of(rows, vocab).parts;
     return stats_bytes(rows, parts) + size_t(rows) * parts * top * 8;
 }
 
 int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int vocab, float scale, const int* given, int n_given,
                         float* given_logprob, float* entropy, int top, int* top_ids, float* top_logprob, void* workspace,
                         size_t workspace_bytes, void* stream) {
-    if (rows < 0 || vocab <= 0 || n_given < 0 || top < 0 || top > kTopMost || top > vocab || !(scale > 0.0f) || !std::isfinite(scale) || pitch < vocab) return 1;
+    if (rows < 0 || vocab <= 0 || vocab > kVocabMost || n_given < 0 || top < 0 || top > kTopMost || top > vocab || !(scale > 0.0f && scale <= kScaleMost) ||
+        pitch < vocab)
+        return 1;
     if (rows == 0) return 0;
     if (!logits || !on(logits, bf16 ? 2 : 4) || (n_given && (!given || !given_logprob || !on(given, 4) || !on(given_logprob, 4))) || !on(entropy, 4) ||
         (top && (!top_ids || !top_logprob || !on(top_ids, 4) || !on(top_logprob, 4))))
         return 1;
     LogprobArgs a{};
-    a.parts = parts_of(rows, vocab);
+    const LogprobCut cut = cut_of(rows, vocab);
+    a.parts = cut.parts;
     const size_t need = m26c_token_logprobs_workspace(rows, vocab, top);
     if (need && (!workspace || !on(workspace, 16) || workspace_bytes < need)) return 1;
     a.logits = logits; a.pitch = pitch; a.rows = rows; a.vocab = vocab; a.scale = scale;
@@ -277,7 +311,7 @@ int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int 
         a.stats = static_cast<float4*>(workspace);
         a.lists = reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + stats_bytes(rows, a.parts));
     }
-    return bf16 ? launch_logprobs<true>(a, hipStream_t(stream)) : launch_logprobs<false>(a, hipStream_t(stream));
+    return bf16 ? launch_logprobs<true>(a, cut.chunks, hipStream_t(stream)) : launch_logprobs<false>(a, cut.chunks, hipStream_t(stream));
 }
 
 }  // extern "C"

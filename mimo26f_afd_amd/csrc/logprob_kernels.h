@@ -174,6 +174,7 @@ struct TopList {
         wave_fence();
         waiting = 0;
     }
+    __device__ __forceinline__ int enough() const { return top < 8 ? 8 : top; }
     // What the values on show vouch for: `top` values of the row reach it, at any ids, so equal ones still count.
     __device__ __forceinline__ void common() {
         const uint32_t v[1] = {__hip_atomic_load(&shown[threadIdx.x & 63], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)};
@@ -184,12 +185,14 @@ struct TopList {
     // when as much waits as the list is to hold: a place costs 50 cycles then, in a list of its own 300.
     __device__ __forceinline__ void take(const float (&v)[8], int id) {
         if (threshold == -INFINITY) {
-            // Nothing known yet: what `top` of the lanes' maxima reach, as many values of this chunk do.
+            // Nothing known yet: what `top` of the lanes' maxima reach, as many values of this chunk do. As many as are put in
+            // their places at once: the few values ahead of a boundary would give a bound that lets half the next chunk pass
+            // (600 x 50003 BF16, top 1: 49 us against 26).
             float largest = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 8; ++j) largest = v[j] > largest ? v[j] : largest;  // a NaN takes no part
             const uint32_t mine[1] = {order_bits(largest)};
-            const uint32_t bound = reached_by<16>(mine, top);
+            const uint32_t bound = reached_by<16>(mine, enough());
             if (bound > order_bits(-INFINITY)) threshold = just_below(order_value(bound));
         }
         // Within the chunk ids are not met in order, so the threshold stays as it is until its end.
@@ -203,7 +206,7 @@ struct TopList {
             if (wanted) batch[waiting + lanes_below(mask)] = list_key(v[j], id + j);
             waiting += n;
         }
-        if (waiting < (top < 8 ? 8 : top)) return;
+        if (waiting < enough()) return;
         const int lane = threadIdx.x & 63;
         merge();
         const uint32_t last = __builtin_amdgcn_readlane(uint32_t(key >> 32), top - 1);
@@ -435,17 +438,19 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
         return sh.count;
     };
     int count = gather();
-    if (count > kRoom) {  // many equal values, or lists that each hold all but one of the largest: the exact cut, bit by bit
+    if (count > kRoom) {  // many equal values, or lists that each hold all but one of the largest: bit by bit, until few enough are left
         bound = 0;
         for (int bit = 63; bit >= 0; --bit) {
             const int n = reach(bound | 1ull << bit);
             if (n && lane == 0) atomicAdd(&sh.reached[bit], n);
             __syncthreads();
-            if (sh.reached[bit] >= a.top) bound |= 1ull << bit;
+            const int all = sh.reached[bit];
+            if (all >= a.top) bound |= 1ull << bit;
+            if (all >= a.top && all <= kRoom) break;
         }
         if (tid == 0) sh.count = 0;
         __syncthreads();
-        count = gather();  // `top`, or all there are
+        count = gather();  // all there are, if that is fewer than `top`
     }
     // a key's place is the number of larger ones
     for (int i = tid; i < count; i += THREADS) {
@@ -520,6 +525,150 @@ __global__ void __launch_bounds__(64 * kPartWaves) logprob_part_kernel(const Log
     if (lane < a.top) a.lists[cell * a.top + lane] = list.key;
 }
 
+// A part of CHUNKS chunks that lie one after another, held in registers: where rows are short or there are few of them, nothing
+// is gained by walking, and what the walk does chunk by chunk (thresholds, merges, two forms of the sums) is done once. The
+// maximum comes first, by comparisons, so the sums are right for any values; the bound is what `top` of the lanes' maxima
+// reach; the few values that reach it are ordered by counting. `batch`: LDS, kBatch, this wave's; put(place, key) takes the list.
+constexpr int kBatch = 128;  // a list of 32 from 1024 values finds about 45 that reach its bound, with 64 places one wave in a thousand goes the long way
+template <bool BF16, int CHUNKS, typename PUT>
+__device__ __forceinline__ SoftmaxSums short_part(const LogprobArgs& a, long row, int part, uint64_t* batch, PUT put) {
+    typedef typename std::conditional<BF16, uint16_t, float>::type T;
+    constexpr int N = 8 * CHUNKS;
+    const int lane = threadIdx.x & 63;
+    const T* base = static_cast<const T*>(a.logits) + row * a.pitch;
+    const int first = part * (CHUNKS * kChunk) + lane * 8;
+    // Chunk i's values of this lane start at id(i); at the row's end they are the last eight, of which the first ones are not its own.
+    auto id = [&](int i) { const int at = first + i * kChunk; return at < a.vocab - 8 ? at : a.vocab - 8; };
+    float v[N];
+    if (a.vocab >= 8) {
+        v4u raw[CHUNKS][BF16 ? 1 : 2];
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+            for (int j = 0; j < (BF16 ? 1 : 2); ++j) raw[i][j] = *(reinterpret_cast<const v4u_any*>(base + id(i)) + j);
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t bits;
+                if constexpr (BF16) bits = j & 1 ? raw[i][0][j / 2] & 0xffff0000u : raw[i][0][j / 2] << 16;
+                else bits = raw[i][j / 4][j % 4];
+                v[8 * i + j] = id(i) + j >= first + i * kChunk ? __uint_as_float(bits) : -INFINITY;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (id(0) + j < first || id(0) + j < 0) continue;
+            if constexpr (BF16) v[j] = __uint_as_float(uint32_t(base[id(0) + j]) << 16);
+            else v[j] = base[id(0) + j];
+        }
+    }
+    const float c = a.scale * 1.44269504088896341f;
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) most = v[i] > most ? v[i] : most;  // a NaN takes no part
+    SoftmaxSums sum;
+    sum.m = wave_max(most);
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum.add(SoftmaxSums::distance(v[i], sum.m, c));
+    sum.z = wave_sum(sum.z);
+    sum.s = wave_sum(sum.s);
+    if (!a.top) return sum;
+    uint32_t order[N];  // 0 for what is no alternative
+#pragma unroll
+    for (int i = 0; i < N; ++i) order[i] = v[i] > -INFINITY ? order_bits(v[i]) : 0;
+    const uint32_t mine[1] = {order_bits(most)};
+    uint32_t cut = reached_by<16>(mine, a.top), id_cut = 0;  // wanted: above the cut, or at it and ~id at least id_cut
+    if (cut == 0) cut = 1;
+    auto wanted = [&](int i) { return order[i] > cut || (order[i] == cut && uint32_t(~(id(i / 8) + i % 8)) >= id_cut); };
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += int(__popcll(__ballot(order[i] >= cut)));
+    if (n > kBatch) {  // many equal values, or too few lanes with any: bit by bit, until few enough are left
+        cut = 0;
+#pragma nounroll
+        for (int bit = 31; bit >= 0 && n > kBatch; --bit) {
+            const uint32_t higher = cut | 1u << bit;
+            int m = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) m += int(__popcll(__ballot(order[i] >= higher)));
+            if (m >= a.top) {
+                cut = higher;
+                n = m;
+            }
+        }
+#pragma nounroll
+        for (int bit = 31; bit >= 0 && n > kBatch; --bit) {  // equal ones by their ids
+            const uint32_t before = id_cut;
+            id_cut |= 1u << bit;
+            int m = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) m += int(__popcll(__ballot(wanted(i))));
+            if (m >= a.top) n = m;
+            else id_cut = before;
+        }
+    }
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bool mine_is = wanted(i);
+        const uint64_t mask = __ballot(mine_is);
+        if (mine_is) batch[at + lanes_below(mask)] = uint64_t(order[i]) << 32 | uint32_t(~(id(i / 8) + i % 8));
+        at += int(__popcll(mask));
+    }
+    wave_fence();
+    auto place = [&](int i) {
+        if (i >= n) {
+            if (i < a.top) put(i, kNoKey);
+            return;
+        }
+        const uint64_t k = batch[i];
+        int larger = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) larger += batch[j] > k;
+        if (larger < a.top) put(larger, k);
+    };
+    place(lane);
+    if (n > 64) place(64 + lane);
+    return sum;
+}
+
+// A workgroup per row at a time, a short part for each of its waves.
+template <bool BF16, int WAVES, int CHUNKS>
+__global__ void __launch_bounds__(64 * WAVES) logprob_short_row_kernel(const LogprobArgs a) {
+    __shared__ float4 sums[WAVES];
+    __shared__ uint64_t batch[WAVES][kBatch], list[WAVES][kTopMost];
+    __shared__ RowShared shared;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const GivenLogit given = given_logit<BF16>(a, row, threadIdx.x);
+        SoftmaxSums sum = short_part<BF16, CHUNKS>(a, row, wave, batch[wave], [&](int place, uint64_t k) { list[wave][place] = k; });
+        if (lane == 0) sums[wave] = make_float4(sum.m, sum.z, sum.s, 0.0f);
+        __syncthreads();
+        if (WAVES > 1) {
+            sum = SoftmaxSums{};
+            if (lane < WAVES) sum = SoftmaxSums{sums[lane].x, sums[lane].y, sums[lane].z};
+            sum.join_lanes(a.scale * 1.44269504088896341f);
+        }
+        const uint64_t key[1] = {lane < a.top ? list[wave][lane] : kNoKey};
+        write_row<BF16, 64 * WAVES>(a, row, sum, given, key, shared);
+        __syncthreads();
+    }
+}
+
+// A row over several workgroups of short parts.
+template <bool BF16, int CHUNKS>
+__global__ void __launch_bounds__(64 * kPartWaves) logprob_short_part_kernel(const LogprobArgs a) {
+    __shared__ uint64_t batch[kPartWaves][kBatch];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long cell = long(blockIdx.x) * kPartWaves + wave;
+    const SoftmaxSums sum = short_part<BF16, CHUNKS>(a, cell / a.parts, int(cell % a.parts), batch[wave],
+                                                     [&](int place, uint64_t k) { a.lists[cell * a.top + place] = k; });
+    if (lane == 0) a.stats[cell] = make_float4(sum.m, sum.z, sum.s, 0.0f);
+}
+
 // ... and a workgroup per row joins them, everything it reads asked for at once.
 constexpr int kJoinThreads = 512;
 template <bool BF16>
@@ -532,14 +681,19 @@ __global__ void __launch_bounds__(kJoinThreads) logprob_join_kernel(const Logpro
     const float4* stats = a.stats + row * a.parts;
     const uint64_t* lists = a.lists + row * a.parts * a.top;
     const GivenLogit given = given_logit<BF16>(a, row, threadIdx.x);
+    // The groups whose maxima give the bound are each a part's list, or with fewer parts each `per`-th key of it: in order over
+    // the threads, groups could hold nothing but last places (1 row x 131072, top 32: 28 us).
+    constexpr int kLanes = kJoinThreads / kGroups;
+    static_assert(kGroups >= kPartsMost && kLanes * N >= kTopMost, "a group takes a whole list");
+    const int per = kGroups / a.parts, group = int(threadIdx.x) / kLanes, part = group / per, sub = group % per;
     float4 two[2];
     uint64_t key[N];
 #pragma unroll
     for (int i = 0; i < 2; ++i) two[i] = lane + 64 * i < a.parts ? stats[lane + 64 * i] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int at = int(threadIdx.x) + kJoinThreads * i;
-        key[i] = at < a.parts * a.top ? lists[at] : kNoKey;
+        const int rank = sub + per * (int(threadIdx.x) % kLanes + kLanes * i);
+        key[i] = part < a.parts && rank < a.top ? lists[part * a.top + rank] : kNoKey;
     }
     SoftmaxSums sum{two[0].x, two[0].y, two[0].z};
     sum.join(SoftmaxSums{two[1].x, two[1].y, two[1].z}, c);

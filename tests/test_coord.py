@@ -73,7 +73,8 @@ def logprob_call(logits=P, bf16=False, rows=2, vocab=100, pitch=100, given=P, n_
 @pytest.mark.parametrize("change", [dict(logits=None), dict(logits=P + 2), dict(logits=P + 1, bf16=True), dict(rows=-1), dict(vocab=0), dict(pitch=99),
                                     dict(given=None), dict(given_logprob=None), dict(n_given=-1), dict(given=P + 2), dict(entropy=P + 1), dict(top=-1),
                                     dict(top=33), dict(top=4, vocab=3), dict(top_ids=None), dict(top_logprob=None), dict(scale=0.0), dict(scale=-1.0),
-                                    dict(scale=float("nan")), dict(scale=float("inf")), dict(rows=1, vocab=131072, pitch=131072, workspace=None),
+                                    dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=2.0 ** 20 * (1 + 2.0 ** -20)),
+                                    dict(vocab=(1 << 30) + 1, pitch=1 << 31), dict(rows=1, vocab=131072, pitch=131072, workspace=None),
                                     dict(rows=1, vocab=131072, pitch=131072, workspace=P + 8),
                                     dict(rows=1, vocab=131072, pitch=131072, workspace_bytes=16)])
 def test_logprobs_refuse(change):
@@ -87,6 +88,15 @@ def test_logprobs_of_no_rows_and_their_workspace():
     need = coord.token_logprobs_workspace(1, 131072, 32)
     assert 0 < need < 1 << 20
     assert coord.token_logprobs_workspace(1, 131072, 33) == 0 and coord.token_logprobs_workspace(1, 131072, -1) == 0
+
+
+def test_logprobs_workspace_bound_for_any_call():
+    """What the header promises, so that a program can set one workspace aside for batches of any size."""
+    sizes = sorted({max(1, (1 << b) + d) for b in range(0, 31) for d in (-1, 0, 1) if (1 << b) + d <= 1 << 30} | {50003, 9000, 8193, 200000, 262144})
+    for vocab in sizes:
+        for rows in (*range(1, 700, 7), 1024, 4096, 8191, 8192, 8193, 1 << 20, (1 << 31) - 1):
+            for top in (0, 1, 32):
+                assert coord.token_logprobs_workspace(rows, vocab, top) <= 8192 * (16 + 8 * top), (rows, vocab, top)
 
 
 def test_join_plan_layout_matches_the_header():

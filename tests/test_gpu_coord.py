@@ -424,7 +424,9 @@ def some_logits(rng, rows, vocab, half, masked=0.0):
 LENGTHS = [(1, 1), (1, 2), (4, 5), (2, 8), (3, 63), (2, 64), (5, 511), (4, 512), (3, 513), (2, 520), (3, 1031), (2, 4099), (40, 2050), (3, 50003), (1, 131072),
            (2, 131075), (1100, 700),
            # every form of the rule on sizes: rows over two, four and eight waves, over several workgroups, more rows than workgroups
-           (1600, 3000), (800, 9000), (600, 9000), (200, 4200), (100, 9000), (5000, 600), (4100, 40), (31, 1537)]
+           (1600, 3000), (800, 9000), (600, 9000), (200, 4200), (100, 9000), (5000, 600), (4100, 40), (31, 1537),
+           # rows in registers, more of them than workgroups; parts of four chunks, the last with values in few lanes; parts that are walked
+           (17000, 40), (1, 1024), (3, 1025), (9, 8192), (9, 8193), (700, 8000), (3, 250000), (2, 262144), (1, 262150), (1, 400001), (90, 100003)]
 
 
 @pytest.mark.parametrize("rows,vocab", LENGTHS)
@@ -442,9 +444,7 @@ def test_logprobs_lengths_starts_and_counts(rows, vocab, half):
         check_logprobs(got, x, given, top, scale)
 
 
-@pytest.mark.parametrize("half", [False, True])
-@pytest.mark.parametrize("vocab", [700, 20011, 131072])
-def test_logprobs_of_rows_that_are_hard_to_select_from(half, vocab):
+def hard_rows(vocab, half):
     """Ties everywhere, values in order either way, one survivor, nothing left, lowest finite values, infinities and NaNs."""
     rng = np.random.default_rng(vocab)
     low = np.float32(R.bf16(np.float32(-3.38e38))[1]) if half else np.finfo(np.float32).min
@@ -478,11 +478,33 @@ def test_logprobs_of_rows_that_are_hard_to_select_from(half, vocab):
     x = R.bf16(x)[1] if half else x
     if half:
         x[np.isnan(np.stack(rows))] = np.nan
+    return x
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("vocab", [700, 2000, 8100, 20011, 131072, 250000])
+def test_logprobs_of_rows_that_are_hard_to_select_from(half, vocab):
+    x = hard_rows(vocab, half)
+    rows = range(len(x))
     given = np.stack([[vocab // 3, 0, vocab - 1]] * len(rows))
     for top in (1, 8, 32):
         check_logprobs(run_logprobs(np.ascontiguousarray(x), given, top, 1.0, half), x.astype(np.float64), given, top, 1.0)
         single = np.concatenate([run_logprobs(x[r:r + 1], given[r:r + 1], top, 1.0, half)[2] for r in range(len(rows))])
         assert np.array_equal(single, run_logprobs(x, given, top, 1.0, half)[2])   # however a row is cut, the same ids
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("vocab,copies,top", [(3001, 120, 8), (3001, 100, 32), (17000, 50, 1), (17000, 50, 20), (17000, 130, 8), (100000, 8, 32)])
+def test_logprobs_of_hard_rows_among_many(half, vocab, copies, top):
+    """The forms that walk over a row, which many rows take. The same row gives the same bits wherever it stands."""
+    x = hard_rows(vocab, half)
+    n = len(x)
+    given = np.stack([[vocab // 3, 0, vocab - 1]] * n)
+    got = run_logprobs(np.tile(x, (copies, 1)), np.tile(given, (copies, 1)), top, 1.0, half, pad=-vocab % 8)
+    check_logprobs([g[:n] for g in got], x.astype(np.float64), given, top, 1.0)
+    for g in got:
+        bits = g.view(np.uint32).reshape(copies, n, -1)
+        assert (bits == bits[:1]).all()
 
 
 def test_logprobs_signalling_nans_do_not_hide_values():
