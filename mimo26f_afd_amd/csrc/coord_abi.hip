@@ -114,43 +114,59 @@ void release(m26c_w4* w) {
     delete w;
 }
 
-template <int TT, int S, int W>
+// Workgroups go round over the eight XCDs. With a multiple of eight of them in a row of the grid, the runs of rows that read the
+// same weights share an L2 (32000 x 8192, 64 rows in four runs: 56 us; with 63 workgroups in a row of the grid 93).
+unsigned over_xcds(int wide, int runs) { return unsigned(runs > 1 ? (wide + 7) / 8 * 8 : wide); }
+
+template <int TT, int S, int W, bool LONG = false>
 int launch_resident(const W4Args& a, int workgroups, int share, hipStream_t st) {
-    const int slices = (a.w.steps + S - 1) / S, groups = W / slices, tiles = (a.w.tiles + groups - 1) / groups;
-    const int turns = (tiles + workgroups - 1) / workgroups, wide = (tiles + turns - 1) / turns;
-    const dim3 grid(unsigned(wide), unsigned((a.rows + share - 1) / share)), block(64, unsigned(slices), unsigned(groups));
-    if (a.y_bf16) w4_resident_kernel<TT, S, W, uint16_t><<<grid, block, 0, st>>>(a, slices, groups, turns, share);
-    else w4_resident_kernel<TT, S, W, float><<<grid, block, 0, st>>>(a, slices, groups, turns, share);
+    const int phases = LONG ? (a.w.steps + W * S - 1) / (W * S) : 1, slices = LONG ? W : (a.w.steps + S - 1) / S, groups = W / slices;
+    const int tiles = (a.w.tiles + groups - 1) / groups;
+    int turns = (tiles + workgroups - 1) / workgroups;
+    if (LONG && turns > kTurnsKept) turns = kTurnsKept;
+    const int wide = (tiles + turns - 1) / turns, runs = (a.rows + share - 1) / share;
+    const dim3 grid(over_xcds(wide, runs), unsigned(runs)), block(64, unsigned(slices), unsigned(groups));
+    if (a.y_bf16) w4_resident_kernel<TT, S, W, LONG, uint16_t><<<grid, block, 0, st>>>(a, slices, groups, turns, phases, share);
+    else w4_resident_kernel<TT, S, W, LONG, float><<<grid, block, 0, st>>>(a, slices, groups, turns, phases, share);
     return launched();
 }
 
 // The form of a product, by sizes alone (us a pass):
 //  * few tiles and rows: a workgroup per tile, rows streamed with the weights. Up to three workgroups per compute unit: 256 tiles
 //    x 32 steps, 1 row 3.9 against 4.9 with resident rows; 626 x 17, 4 rows 5.2 against 6.0; 1024 x 32, 16 rows 10.6
-//    against 9.7 the other way. Also where k is past what registers hold (64 steps).
-//  * otherwise resident rows: sixteen a workgroup, or 32 where a wave's slice of them fits (1024 tiles x 32 steps, 64 rows: 17.8
-//    against 22.3), one workgroup per compute unit over all row runs, so that each loads its rows once.
-//    Sixteen waves hold up to 64 steps (8192 tiles x 32 steps: 48.3 us with sixteen waves of two steps, 50.1 with eight of four);
-//    up to sixteen steps eight waves do, twice as many workgroups up to eight steps (2048 x 8: 7.8 against 8.9).
+//    against 9.7 the other way. Eight waves, a step at a time: sixteen lose where tiles meet on a compute unit (626 x 17 of wire
+//    rows 9.4 against 7.0), and so do two steps on their way (6.8 against 6.3), which gain on long k (125 x 128, 16 rows 9.8
+//    against 11.4; 256 x 64, 1 row 6.3 against 7.1).
+//  * otherwise resident rows, one workgroup per compute unit over all row runs, so that each loads its rows once. Sixteen waves
+//    hold sixteen rows up to 64 steps (8192 tiles x 32 steps: 48.3 us with sixteen waves of two steps, 50.1 with eight of
+//    four) and 32 rows up to 32 (1024 x 32, 64 rows: 17.8 against 22.3 with 16 a run); up to sixteen steps eight waves do, twice as
+//    many workgroups up to eight steps (2048 x 8: 7.8 against 8.9). Past 64 steps in phases, again 32 rows a run (1875 x
+//    80, 64 rows: 88 against 110), but from 33 to 64 sixteen, which need none (2000 x 64, 64 rows: 56 against 68).
 int launch_w4(const W4Args& a, hipStream_t st) {
     const int steps = a.w.steps, runs16 = (a.rows + 15) / 16;
-    if (steps > 64 || long(a.w.tiles) * runs16 <= 768) {
+    if (long(a.w.tiles) * runs16 <= 768) {
         const int share = (a.rows + runs16 - 1) / runs16;
-        w4_streamed_kernel<<<dim3(unsigned(a.w.tiles), unsigned(runs16)), 512, 0, st>>>(a, share);
+        const dim3 grid(over_xcds(a.w.tiles, runs16), unsigned(runs16));
+        if (steps >= 64) w4_streamed_kernel<8, 2><<<grid, 512, 0, st>>>(a, share);
+        else w4_streamed_kernel<8, 1><<<grid, 512, 0, st>>>(a, share);
         return launched();
     }
-    const int runs = a.rows > 16 && steps <= 32 ? (a.rows + 31) / 32 : runs16, share = (a.rows + runs - 1) / runs;
+    const int runs = a.rows > 16 && (steps <= 32 || steps > 64) ? (a.rows + 31) / 32 : runs16, share = (a.rows + runs - 1) / runs;
     const int workgroups = runs < 256 ? 256 / runs : 1;
     if (share > 16) {
         if (steps <= 8) return launch_resident<2, 1, 8>(a, 2 * workgroups, share, st);
         if (steps <= 16) return launch_resident<2, 2, 8>(a, workgroups, share, st);
-        return launch_resident<2, 2, 16>(a, workgroups, share, st);
+        if (steps <= 32) return launch_resident<2, 2, 16>(a, workgroups, share, st);
+        return launch_resident<2, 2, 16, true>(a, workgroups, share, st);
     }
     if (steps <= 8) return launch_resident<1, 1, 8>(a, 2 * workgroups, share, st);
     if (steps <= 16) return launch_resident<1, 2, 8>(a, workgroups, share, st);
     if (steps <= 32) return launch_resident<1, 2, 16>(a, workgroups, share, st);
     if (steps <= 48) return launch_resident<1, 3, 16>(a, workgroups, share, st);
-    return launch_resident<1, 4, 16>(a, workgroups, share, st);
+    if (steps <= 64) return launch_resident<1, 4, 16>(a, workgroups, share, st);
+    const int threes = (steps + 47) / 48 * 3, fours = (steps + 63) / 64 * 4;  // steps a wave goes through
+    if (threes < fours) return launch_resident<1, 3, 16, true>(a, workgroups, share, st);
+    return launch_resident<1, 4, 16, true>(a, workgroups, share, st);
 }
 
 int w4_run(const m26c_w4* w, W4Args a, bool fp8, void* stream) {

@@ -88,6 +88,7 @@ __device__ __forceinline__ v8bf w4_widen(uint32_t codes, float scale) {
     return u.all;
 }
 
+typedef uint32_t u32_any __attribute__((aligned(1)));
 typedef uint32_t v2u32 __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u32 __attribute__((ext_vector_type(4)));
 
@@ -114,20 +115,29 @@ struct W4Rows {
         const int lane = threadIdx.x & 63, q = lane >> 4, c = lane & 15;
         if (a.fp8) {
             const __amdgpu_buffer_rsrc_t codes = w4_run_of(a.x_codes + row0 * a.x_pitch, kRunMost);
-            const __amdgpu_buffer_rsrc_t bytes = w4_run_of(a.x_scales + row0 * a.x_scales_pitch, kRunMost);
+            const int groups = int(a.w.k / 32);
             v2u32 raw[STEPS][TT][4];
-            uint32_t scale[STEPS][TT][4];
+            uint32_t scale[STEPS][TT];  // a step's four bytes of a row at once, at any alignment: byte by byte they took longer than the codes (16 rows x 4096 to 256: 7.0 us)
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                for (int t = 0; t < TT; ++t)
+                for (int t = 0; t < TT; ++t) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int row = 16 * t + 4 * i + q, group = (step0 + s) * 4 + i;
-                        const bool there = row < rows && (step0 + s) * 128 + c * 8 < a.w.k, group_there = 16 * t + c < rows && group * 32 < a.w.k;
+                        const int row = 16 * t + 4 * i + q;
+                        const bool there = row < rows && (step0 + s) * 128 + c * 8 < a.w.k;
                         raw[s][t][i] = __builtin_amdgcn_raw_buffer_load_b64(codes, there ? row * int(a.x_pitch) + c * 8 : kOutside, (step0 + s) * 128, 0);
-                        scale[s][t][i] = __builtin_amdgcn_raw_buffer_load_b8(bytes, group_there ? (16 * t + c) * int(a.x_scales_pitch) : kOutside, group, 0);
                     }
+                    // Rows that are not there take the last one's. At the row's end the last four bytes, moved down; past k the codes are zero.
+                    const int row = 16 * t + c < rows ? 16 * t + c : rows - 1, group = (step0 + s) * 4;
+                    const uint8_t* bytes = a.x_scales + (row0 + row) * a.x_scales_pitch;
+                    if (groups >= 4) {
+                        const int at = group + 4 <= groups ? group : groups - 4, past = group - at < 4 ? group - at : 0;
+                        scale[s][t] = *reinterpret_cast<const u32_any*>(bytes + at) >> (8 * past);
+                    } else {
+                        scale[s][t] = bytes[0] | (groups > 1 ? bytes[1] << 8 : 0) | (groups > 2 ? bytes[2] << 16 : 0);
+                    }
+                }
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
@@ -137,7 +147,7 @@ struct W4Rows {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const v2u32 code = *reinterpret_cast<const v2u32*>(corner + c * kTurnRow + i * 32 + q * 8);
-                        const uint32_t byte = scale[s][t][i];
+                        const uint32_t byte = scale[s][t] >> (8 * i) & 0xffu;
                         const float f = __uint_as_float((byte ? byte : 1u) << 23);  // byte 0 marks a block of zeros
                         union { v2bf pair[4]; v8bf all; uint32_t dword[4]; } u;
                         u.pair[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code.x, f, false);
@@ -179,54 +189,64 @@ struct W4Rows {
 __device__ __forceinline__ float w4_scale(uint32_t dword, int i) { return __uint_as_float((dword >> (8 * i) & 0xffu) << 23); }
 
 // Rows resident: x stays in registers. A workgroup's waves are `groups` column groups of `slices` k-slices, S steps each;
-// a wave converts its slice of 16 * TT rows to matrix operands once and then walks over the tiles, DEPTH of them in flight,
+// a wave converts its slice of 16 * TT rows to matrix operands once and then walks over the tiles, the next one on its way,
 // with nothing but weights left to load. The slices' sums meet in LDS, in order, two buffers taking turns so that one
 // barrier per turn does. A workgroup's tiles are neighbours, so that what it writes of a row grows into whole 256-byte
 // pieces in its L2 (16 rows x 131072 columns from 131072 x 4096: 50 us; with a workgroup's tiles a grid apart, 64 bytes
 // of a row from each XCD in turn, 55). Tiles past the last load and store nothing. blockIdx.y is a run of `share` rows.
-template <int TT, int S, int W, typename OUT>
-__global__ void __launch_bounds__(64 * W, W / 4) w4_resident_kernel(const W4Args a, int slices, int groups, int turns, int share) {
+//
+// Where the registers do not hold x's whole width (LONG, one column group of W slices), it goes in phases of W * S steps: a
+// phase loads its part of x, walks over all tiles, and the sums so far wait in LDS. Streaming x with the weights instead moves
+// it once a tile (16 rows, 32768 x 16384: 93 us against 49, 6.0 TB/s).
+constexpr int kTurnsKept = 32;
+template <int TT, int S, int W, bool LONG, typename OUT>
+__global__ void __launch_bounds__(64 * W, W / 4) w4_resident_kernel(const W4Args a, int slices, int groups, int turns, int phases, int share) {
     // Each wave's corner while x is turned round, the slices' sums afterwards.
     constexpr int kSums = 2 * W * TT * 256 * 4;
     __shared__ __attribute__((aligned(16))) uint8_t shared[kSums > W * kTurnBytes ? kSums : W * kTurnBytes];
+    __shared__ float kept[LONG ? kTurnsKept : 1][TT * 256];  // each cell by one thread
     float (*sums)[W][TT][256] = reinterpret_cast<float (*)[W][TT][256]>(shared);
     // a workgroup is (64 lanes, slices, groups)
     const int lane = threadIdx.x, q = lane >> 4;
     const int slice = __builtin_amdgcn_readfirstlane(threadIdx.y), group = __builtin_amdgcn_readfirstlane(threadIdx.z), wave = group * slices + slice;
     const int row0 = blockIdx.y * share, rows = a.rows - row0 < share ? a.rows - row0 : share, threads = groups * slices * 64;
     auto tile_of = [&](int turn) { return turn < turns ? (int(blockIdx.x) * turns + turn) * groups : a.w.tiles; };  // of column group 0
+    if (tile_of(0) >= a.w.tiles) return;  // the grid is rounded up
     const uint32_t step_bytes = uint32_t(a.w.steps) * 1024, scale_bytes = uint32_t(a.w.quads) * 256;
     struct Tile {
         v4u32 codes[S];
         uint32_t scales[S];
     };
-    auto load = [&](int tile, Tile& t) {
+    auto load = [&](int tile, int phase, Tile& t) {
+        const int step0 = phase * (W * S) + slice * S;
         const bool there = tile < a.w.tiles;
         const long at = there ? tile : 0;
         const __amdgpu_buffer_rsrc_t codes = w4_run_of(a.payload + at * step_bytes, there ? step_bytes : 0);
         const __amdgpu_buffer_rsrc_t scales = w4_run_of(reinterpret_cast<const uint8_t*>(a.scales) + at * scale_bytes, there ? scale_bytes : 0);
 #pragma unroll
-        for (int s = 0; s < S; ++s) t.codes[s] = __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, (slice * S + s) * 1024, kStreamed);
+        for (int s = 0; s < S; ++s) t.codes[s] = __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16, (step0 + s) * 1024, kStreamed);
         // a dword per step and column; four steps of a quad lie together
         if constexpr (S % 4 == 0) {
 #pragma unroll
             for (int s = 0; s < S; s += 4) {
-                const v4u32 v = __builtin_amdgcn_raw_buffer_load_b128(scales, (lane & 15) * 16, (slice * S + s) * 64, kStreamed);
+                const v4u32 v = __builtin_amdgcn_raw_buffer_load_b128(scales, (lane & 15) * 16, (step0 + s) * 64, kStreamed);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) t.scales[s + j] = v[j];
             }
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const int step = slice * S + s;
+                const int step = step0 + s;
                 t.scales[s] = __builtin_amdgcn_raw_buffer_load_b32(scales, (lane & 15) * 16, (step >> 2) * 256 + (step & 3) * 4, kStreamed);
             }
         }
     };
     Tile ahead;
-    load(tile_of(0) + group, ahead);
+    load(tile_of(0) + group, 0, ahead);
+    for (int phase = 0; phase < (LONG ? phases : 1); ++phase) {
+    if (phase) __syncthreads();  // the last turn's sums are read
     W4Rows<S, TT> x;
-    x.load(a, row0, rows, slice * S, shared + wave * kTurnBytes);
+    x.load(a, row0, rows, phase * (W * S) + slice * S, shared + wave * kTurnBytes);
     __syncthreads();
     for (int turn = 0; turn < turns; ++turn) {  // the same for every wave
         const int tile = tile_of(turn);
@@ -241,7 +261,9 @@ __global__ void __launch_bounds__(64 * W, W / 4) w4_resident_kernel(const W4Args
 #pragma unroll
                 for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, x.part[s][t][i], acc[t], 0, 0, 0);
             }
-        load(tile_of(turn + 1) + group, ahead);  // under the sums and stores of this one
+        // under the sums and stores of this one
+        if (LONG && turn + 1 == turns && phase + 1 < phases) load(tile_of(0) + group, phase + 1, ahead);
+        else load(tile_of(turn + 1) + group, phase, ahead);
         float (*mine)[TT][256] = sums[turn & 1];
 #pragma unroll
         for (int t = 0; t < TT; ++t) *reinterpret_cast<v4f32*>(&mine[wave][t][(lane & 15) * 16 + 4 * q]) = acc[t];
@@ -256,6 +278,11 @@ __global__ void __launch_bounds__(64 * W, W / 4) w4_resident_kernel(const W4Args
                 const float part = mine[g * slices + (w < slices ? w : 0)][t][cell];
                 s += w < slices ? part : 0.0f;
             }
+            if (LONG) {
+                if (phase) s += kept[turn][i];
+                kept[turn][i] = s;
+                if (phase + 1 < phases) continue;
+            }
             const int at = (r * int(a.y_pitch) + c) * int(sizeof(OUT));
             if (r < rows && c < left) {
                 if constexpr (sizeof(OUT) == 2) __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bf16_rne_nan(s)), y, at, 0, 0);
@@ -263,36 +290,39 @@ __global__ void __launch_bounds__(64 * W, W / 4) w4_resident_kernel(const W4Args
             }
         }
     }
+    }
 }
 
-// Rows streamed: a workgroup of eight waves takes one tile of sixteen columns and `share` <= 16 rows; the waves take the
-// tile's quads of k-steps in turn, weights and rows alike, and their sums meet in LDS, in wave order. A step at a time: with a
-// quad's sixteen loads of x ahead of its products a wave holds twice the registers, and where two or three tiles meet on a
-// compute unit that costs more than it hides (626 tiles x 17 steps 8.5 against 6.6 us, 256 x 32 4.0 against 3.9).
-__global__ void __launch_bounds__(512) w4_streamed_kernel(const W4Args a, int share) {
-    constexpr int WAVES = 8;
+// Rows streamed: a workgroup takes one tile of sixteen columns and `share` <= 16 rows; its waves take the tile's k-steps in
+// turn, weights and rows alike, AHEAD of them on their way at once, and their sums meet in LDS, in wave order.
+template <int WAVES, int AHEAD>
+__global__ void __launch_bounds__(64 * WAVES) w4_streamed_kernel(const W4Args a, int share) {
     __shared__ float sums[WAVES][256];
     __shared__ __attribute__((aligned(16))) uint8_t corners[WAVES][kTurnBytes];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4;
     const long tile = blockIdx.x, row0 = long(blockIdx.y) * share;
+    if (tile >= a.w.tiles) return;  // the grid is rounded up
     const int rows = a.rows - row0 < share ? int(a.rows - row0) : share;
     const uint4* payload = reinterpret_cast<const uint4*>(a.payload) + tile * a.w.steps * 64 + lane;
-    const uint4* scales = reinterpret_cast<const uint4*>(a.scales) + tile * a.w.quads * 16 + (lane & 15);
+    const uint32_t* scales = a.scales + tile * a.w.quads * 64 + (lane & 15) * 4;
     v4f32 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int quad = wave; quad < a.w.quads; quad += WAVES) {
-        const uint4 four = scales[quad * 16];
-        const uint32_t scale[4] = {four.x, four.y, four.z, four.w};
+    for (int first = wave * AHEAD; first < a.w.steps; first += WAVES * AHEAD) {
+        uint4 codes[AHEAD];
+        uint32_t scale[AHEAD];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const int step = quad * 4 + s;
-            if (step >= a.w.steps) break;  // the same for the whole workgroup
-            const uint4 codes = payload[step * 64];
-            const uint32_t dword[4] = {codes.x, codes.y, codes.z, codes.w};
-            W4Rows<1, 1> x;
-            x.load(a, row0, rows, step, corners[wave]);
+        for (int s = 0; s < AHEAD; ++s) {
+            const int step = first + s < a.w.steps ? first + s : a.w.steps - 1;
+            codes[s] = payload[step * 64];
+            scale[s] = scales[(step >> 2) * 64 + (step & 3)];
+        }
+        W4Rows<AHEAD, 1> x;  // zeros past k
+        x.load(a, row0, rows, first, corners[wave]);
+#pragma unroll
+        for (int s = 0; s < AHEAD; ++s) {
+            const uint32_t dword[4] = {codes[s].x, codes[s].y, codes[s].z, codes[s].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w4_widen(dword[i], w4_scale(scale[s], i)), x.part[0][0][i], acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w4_widen(dword[i], w4_scale(scale[s], i)), x.part[s][0][i], acc, 0, 0, 0);
         }
     }
     *reinterpret_cast<v4f32*>(&sums[wave][(lane & 15) * 16 + 4 * q]) = acc;  // [row][column of the tile]

@@ -243,7 +243,7 @@ SHAPES = [(1, 1, 32), (1, 16, 64), (3, 17, 96), (16, 256, 4096), (17, 100, 128),
           (1, 4096, 4096), (2, 5, 16384), (48, 4099, 608), (16, 33000, 256),
           # every form of the rule on sizes: steps of 128 up to 8, 16, 24, 32, 48, 64 and more, in runs of 16 and 32 rows, tiles past one turn
           (3, 13000, 1056), (16, 12500, 2080), (9, 12400, 3200), (7, 12400, 4128), (5, 12330, 6176), (2, 12330, 8224), (33, 8200, 96), (29, 13000, 1056),
-          (64, 8200, 2080), (50, 4200, 3200), (64, 4200, 4128), (300, 200, 640), (2, 40, 16416)]
+          (64, 8200, 2080), (50, 4200, 3200), (64, 4200, 4128), (300, 200, 640), (2, 40, 16416), (33, 3104, 16416), (1, 1, 64), (3, 7, 96)]
 
 
 @pytest.mark.parametrize("rows,n,k", SHAPES)
@@ -267,6 +267,34 @@ def test_w4_product_within_counted_roundings(rows, n, k, form):
     assert np.array_equal(padded.view(np.uint32), got.view(np.uint32))
     half = run(bf16_out=True)
     assert np.array_equal(half, R.bf16(got)[1])
+
+
+@pytest.mark.parametrize("rows,n,k", [(3, 12400, 12320), (16, 12301, 16384), (40, 70001, 8224), (17, 13000, 8224)])
+@pytest.mark.parametrize("form", ["bf16", "fp8"])
+def test_w4_wide_rows_in_phases(rows, n, k, form):
+    """x too wide for the registers over many columns, and more tiles than a workgroup keeps sums for; the reference takes every 61st
+    column and the last ones; with a single one in each row of weights every column is pinned."""
+    rng, payload, scales = w4_inputs(n, k, rows + n)
+    weights = weights_of(payload, scales)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    if form == "bf16":
+        bits, value = R.bf16(x)
+        got = run_w4(weights, bits, rows, y_pad=5)
+    else:
+        wire = O.q0_quantize(x)
+        value = R.wire_values(*wire)
+        got = run_w4(weights, None, rows, fp8=wire, y_pad=5)
+    some = np.unique(np.r_[0:n:61, n - 20:n])
+    want, tol = R.w4_product(value, R.w4_weights(payload[some], scales[some]))
+    assert np.all(np.abs(got[:, some] - want) <= tol), np.max(np.abs(got[:, some] - want) / tol)
+    # one in each row of weights, at a place that depends on the column: y names x's value there
+    weights.close()
+    place = (np.arange(n) * 7919) % k
+    payload = np.zeros((n, k // 2), np.uint8)
+    payload[np.arange(n), place // 2] = 2 << (4 * (place % 2))
+    weights = weights_of(payload, np.full((n, k // 32), 127, np.uint8))
+    got = run_w4(weights, bits, rows) if form == "bf16" else run_w4(weights, None, rows, fp8=wire)
+    assert np.array_equal(got, value[:, place].astype(np.float32))
 
 
 def test_w4_product_is_exact_on_small_integers():
