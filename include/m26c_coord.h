@@ -54,8 +54,8 @@ int m26c_block_join(const m26c_join* plan, long rows, const float* h, const uint
 /* ---- products with MXFP4 weights -----------------------------------------------------------------------
  * y[r][j] = sum over k of x[r][k] * e2m1(code[j][k]) * 2^(scale[j][k / 32] - 127)
  * Weights in the checkpoint's own form: [n][k / 2] payload bytes, low nibble = even k, [n][k / 32] scale bytes;
- * k a multiple of 32, n and k up to 2^24, and so are the pitches of x and y. m26c_w4_new lays them out once in the order the matrix pipe reads, on the current device, and
- * waits for that; the sources may be freed afterwards. Scale bytes have to lie in [2, 252] wherever a group holds a
+ * k a multiple of 32, n and k up to 2^24, and so are the pitches of x and y. m26c_w4_new lays them out once in the order the
+ * matrix pipe reads, on the current device, and waits for that; the sources may be freed afterwards. Scale bytes have to lie in [2, 252] wherever a group holds a
  * nonzero code (the format's range in which every product is a normal number); a group of zeros may carry any byte.
  * Returns 1 for a bad argument, 2 for a failed allocation or launch, 3 for a scale byte out of that range. */
 typedef struct m26c_w4 m26c_w4;
@@ -64,7 +64,7 @@ void m26c_w4_free(m26c_w4* w);
 
 /* x: BF16 rows at x_pitch elements, 16-byte aligned and the pitch a multiple of 8. y: FP32, or BF16 (nearest even) when
  * y_bf16 is not 0, rows at y_pitch elements. Sums are FP32. Made for up to 64 rows; any number is
- * taken, 32 at a time. The current device has to be the one the weights are on. */
+ * taken, 16 or 32 at a time. The current device has to be the one the weights are on. */
 int m26c_w4_matvec(const m26c_w4* w, const uint16_t* x, long x_pitch, int rows, void* y, int y_bf16, long y_pitch, void* stream);
 
 /* The same on wire rows: E4M3 codes and one UE8M0 byte per 32 values, at their own pitches in bytes (request-frame rows are

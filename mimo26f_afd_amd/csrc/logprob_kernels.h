@@ -3,17 +3,21 @@
 //   Z = sum exp(t - m),  S = sum exp(t - m) (t - m)
 //   log p(j) = t_j - m - ln Z,   entropy = ln Z - S / Z,   the largest logits in descending order, equal ones by the lower id
 //
-// The logits are read once, which is the bound: everything else is a few values per row. About nine vector instructions a
-// value (one of them an exponential) are four fifths of what the chip does in the time HBM needs for a BF16 value, so the
-// selection may add next to nothing to the common path.
+// The logits are read once, which is the bound of large calls: everything else is a few values per row. About nine vector
+// instructions a value (one of them an exponential) are four fifths of what the chip does in the time HBM needs for a BF16
+// value, so the selection may add next to nothing to the common path: 2048 rows x 131072 BF16, top 5, 537 MB in 96 us (5.6
+// TB/s, 84 % of a streaming read). Small calls are chains of dependent steps: 1 row x 131072 9.8 us, two launches 4 of them.
+//
+// Two forms. Many long rows are walked, as follows; few rows or short ones are held in registers (short_part below).
 //
 // Selection. A wave keeps its part's largest values in order, one to a lane, and walks the part in ascending order, 512 values
 // at a time, with the top-th of them as a threshold. Values above it wait in LDS until there are as many as the list is to
 // hold and are put in their places together; an equal one need not be: `top` values of its size with lower ids are there. One
 // comparison of each lane's maximum, which the softmax needs anyway, and a scalar branch are the whole cost where nothing
-// qualifies, which after i chunks is all but about top / i of them. The waves of a workgroup help each other: of the 64 values that they have on show, the
-// largest of each, the top-th largest is a bound that `top` values of the row reach. List entries are 64-bit keys, the value's bits in integer order above the
-// complemented id: a total order, so the result does not depend on who finds what when.
+// qualifies, which after i chunks is all but about top / i of them. The waves of a workgroup help each other: of the 64 values
+// that they have on show, the largest of each, the top-th largest is a bound that `top` values of the row reach. List entries
+// are 64-bit keys, the value's bits in integer order above the complemented id: a total order, so the result does not depend
+// on who finds what when.
 //
 // A row is cut into parts, a wave each, whose chunks lie side by side. The parts' lists meet in one workgroup: their keys in
 // 128 groups, the top-th largest of the groups' maxima is a bound that `top` keys reach and few others, and what reaches it is
@@ -400,75 +404,75 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
             }
         }
     } else {
-    // The bound: values alone, from the maxima of kGroups groups of threads.
-    constexpr int kLanes = THREADS / kGroups;  // of a group
-    static_assert(THREADS % kGroups == 0 && kLanes <= 8, "the lanes' exchanges below");
-    uint32_t most = 0;
+        // The bound: values alone, from the maxima of kGroups groups of threads.
+        constexpr int kLanes = THREADS / kGroups;  // of a group
+        static_assert(THREADS % kGroups == 0 && kLanes <= 8, "the lanes' exchanges below");
+        uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) most = uint32_t(key[i] >> 32) > most ? uint32_t(key[i] >> 32) : most;
-    auto larger_of = [&](uint32_t o) { most = o > most ? o : most; };
-    if (kLanes > 1) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kQuadXor1, 0xf, 0xf, false)));
-    if (kLanes > 2) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kQuadXor2, 0xf, 0xf, false)));
-    if (kLanes > 4) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kHalfRowMirror, 0xf, 0xf, false)));
-    if (tid % kLanes == 0) sh.most[tid / kLanes] = most;
-    if (tid >= THREADS - 64) sh.reached[lane] = 0;
-    if (tid == 64) sh.count = 0;
-    __syncthreads();
-    const uint32_t two[2] = {sh.most[lane], sh.most[64 + lane]};
-    uint64_t bound = uint64_t(reached_by<16>(two, a.top)) << 32;
-    auto reach = [&](uint64_t k) {  // keys of this wave that reach k
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < N; ++i) n += int(__popcll(__ballot(key[i] != kNoKey && key[i] >= k)));
-        return n;
-    };
-    auto gather = [&] {  // a key's place in the result does not depend on which wave is first here
-        const int here = reach(bound);
-        int at = 0;
-        if (here && lane == 0) at = atomicAdd(&sh.count, here);
-        at = __builtin_amdgcn_readfirstlane(at);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const bool kept = key[i] != kNoKey && key[i] >= bound;
-            const uint64_t mask = __ballot(kept);
-            if (kept && at + lanes_below(mask) < kRoom) sh.room[at + lanes_below(mask)] = key[i];
-            at += int(__popcll(mask));
-        }
+        for (int i = 0; i < N; ++i) most = uint32_t(key[i] >> 32) > most ? uint32_t(key[i] >> 32) : most;
+        auto larger_of = [&](uint32_t o) { most = o > most ? o : most; };
+        if (kLanes > 1) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kQuadXor1, 0xf, 0xf, false)));
+        if (kLanes > 2) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kQuadXor2, 0xf, 0xf, false)));
+        if (kLanes > 4) larger_of(uint32_t(__builtin_amdgcn_update_dpp(0, int(most), kHalfRowMirror, 0xf, 0xf, false)));
+        if (tid % kLanes == 0) sh.most[tid / kLanes] = most;
+        if (tid >= THREADS - 64) sh.reached[lane] = 0;
+        if (tid == 64) sh.count = 0;
         __syncthreads();
-        return sh.count;
-    };
-    int count = gather();
-    if (count > kRoom) {  // many equal values, or lists that each hold all but one of the largest: bit by bit, until few enough are left
-        bound = 0;
-        for (int bit = 63; bit >= 0; --bit) {
-            const int n = reach(bound | 1ull << bit);
-            if (n && lane == 0) atomicAdd(&sh.reached[bit], n);
+        const uint32_t two[2] = {sh.most[lane], sh.most[64 + lane]};
+        uint64_t bound = uint64_t(reached_by<16>(two, a.top)) << 32;
+        auto reach = [&](uint64_t k) {  // keys of this wave that reach k
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) n += int(__popcll(__ballot(key[i] != kNoKey && key[i] >= k)));
+            return n;
+        };
+        auto gather = [&] {  // a key's place in the result does not depend on which wave is first here
+            const int here = reach(bound);
+            int at = 0;
+            if (here && lane == 0) at = atomicAdd(&sh.count, here);
+            at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const bool kept = key[i] != kNoKey && key[i] >= bound;
+                const uint64_t mask = __ballot(kept);
+                if (kept && at + lanes_below(mask) < kRoom) sh.room[at + lanes_below(mask)] = key[i];
+                at += int(__popcll(mask));
+            }
             __syncthreads();
-            const int all = sh.reached[bit];
-            if (all >= a.top) bound |= 1ull << bit;
-            if (all >= a.top && all <= kRoom) break;
+            return sh.count;
+        };
+        int count = gather();
+        if (count > kRoom) {  // many equal values, or lists that each hold all but one of the largest: bit by bit, until few enough are left
+            bound = 0;
+            for (int bit = 63; bit >= 0; --bit) {
+                const int n = reach(bound | 1ull << bit);
+                if (n && lane == 0) atomicAdd(&sh.reached[bit], n);
+                __syncthreads();
+                const int all = sh.reached[bit];
+                if (all >= a.top) bound |= 1ull << bit;
+                if (all >= a.top && all <= kRoom) break;
+            }
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            count = gather();  // all there are, if that is fewer than `top`
         }
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        count = gather();  // all there are, if that is fewer than `top`
-    }
-    // a key's place is the number of larger ones
-    for (int i = tid; i < count; i += THREADS) {
-        const uint64_t k = sh.room[i];
-        int larger = 0, j = 0;
-        for (; j + 8 <= count; j += 8)
+        // a key's place is the number of larger ones
+        for (int i = tid; i < count; i += THREADS) {
+            const uint64_t k = sh.room[i];
+            int larger = 0, j = 0;
+            for (; j + 8 <= count; j += 8)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) larger += sh.room[j + u] > k;
-        for (; j < count; ++j) larger += sh.room[j] > k;
-        if (larger < a.top) {
-            a.top_ids[row * a.top + larger] = key_id(k);
-            a.top_logprob[row * a.top + larger] = logprob(key_value(k));
+                for (int u = 0; u < 8; ++u) larger += sh.room[j + u] > k;
+            for (; j < count; ++j) larger += sh.room[j] > k;
+            if (larger < a.top) {
+                a.top_ids[row * a.top + larger] = key_id(k);
+                a.top_logprob[row * a.top + larger] = logprob(key_value(k));
+            }
         }
-    }
-    for (int p = count + tid; p < a.top; p += THREADS) {
-        a.top_ids[row * a.top + p] = -1;
-        a.top_logprob[row * a.top + p] = -INFINITY;
-    }
+        for (int p = count + tid; p < a.top; p += THREADS) {
+            a.top_ids[row * a.top + p] = -1;
+            a.top_logprob[row * a.top + p] = -INFINITY;
+        }
     }
 }
 
@@ -529,7 +533,9 @@ __global__ void __launch_bounds__(64 * kPartWaves) logprob_part_kernel(const Log
 // is gained by walking, and what the walk does chunk by chunk (thresholds, merges, two forms of the sums) is done once. The
 // maximum comes first, by comparisons, so the sums are right for any values; the bound is what `top` of the lanes' maxima
 // reach; the few values that reach it are ordered by counting. `batch`: LDS, kBatch, this wave's; put(place, key) takes the list.
-constexpr int kBatch = 128;  // a list of 32 from 1024 values finds about 45 that reach its bound, with 64 places one wave in a thousand goes the long way
+// About 45 of 1024 values reach the bound of a list of 32; with 64 places some wave of many goes the long way (4096 x 1000 BF16:
+// 25 us against 11).
+constexpr int kBatch = 128;
 template <bool BF16, int CHUNKS, typename PUT>
 __device__ __forceinline__ SoftmaxSums short_part(const LogprobArgs& a, long row, int part, uint64_t* batch, PUT put) {
     typedef typename std::conditional<BF16, uint16_t, float>::type T;

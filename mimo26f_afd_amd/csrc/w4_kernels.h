@@ -6,7 +6,8 @@
 // are widened to BF16 in registers (v_cvt_scalef32_pk_bf16_fp4: two values and the group's scale in one instruction,
 // exact for scale bytes 2..252) and multiplied on v_mfma_f32_16x16x32_bf16, whose products of BF16 values are exact and
 // whose sums are FP32. One 16-column tile's 128 k take 1 KB of codes, 16 conversions and, per 16 rows, 4 MFMAs of 16 cycles
-// on one of a compute unit's four SIMDs; at 6.5 TB/s such a kilobyte arrives every 96 cycles per compute unit.
+// on one of a compute unit's four SIMDs; at 6.5 TB/s such a kilobyte arrives every 96 cycles per compute unit. 16 rows,
+// 131072 x 4096: 48 us, 6.1 TB/s; 64 rows, 16384 x 4096: 16.5 us, of which fetching x takes 2.7, joining the slices' sums 2.6.
 //
 // Operand order. v_mfma_f32_16x16x32_bf16: lane l holds row (l % 16) of either operand, eight k values of quarter
 // (l / 16); the result's lane l holds D[4 * (l / 16) + i][l % 16]. A 128-wide k-step is four MFMAs, one per group of 32, and a
@@ -117,7 +118,9 @@ struct W4Rows {
             const __amdgpu_buffer_rsrc_t codes = w4_run_of(a.x_codes + row0 * a.x_pitch, kRunMost);
             const int groups = int(a.w.k / 32);
             v2u32 raw[STEPS][TT][4];
-            uint32_t scale[STEPS][TT];  // a step's four bytes of a row at once, at any alignment: byte by byte they took longer than the codes (16 rows x 4096 to 256: 7.0 us)
+            // A step's four bytes of a row at once, at any alignment: byte by byte they took longer than the codes (16 rows, 256 x
+            // 4096: 7.0 us against 4.6).
+            uint32_t scale[STEPS][TT];
 #pragma unroll
             for (int s = 0; s < STEPS; ++s)
 #pragma unroll
@@ -244,52 +247,52 @@ __global__ void __launch_bounds__(64 * W, W / 4) w4_resident_kernel(const W4Args
     Tile ahead;
     load(tile_of(0) + group, 0, ahead);
     for (int phase = 0; phase < (LONG ? phases : 1); ++phase) {
-    if (phase) __syncthreads();  // the last turn's sums are read
-    W4Rows<S, TT> x;
-    x.load(a, row0, rows, phase * (W * S) + slice * S, shared + wave * kTurnBytes);
-    __syncthreads();
-    for (int turn = 0; turn < turns; ++turn) {  // the same for every wave
-        const int tile = tile_of(turn);
-        v4f32 acc[TT];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) acc[t] = v4f32{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < S; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const v8bf wide = w4_widen(ahead.codes[s][i], w4_scale(ahead.scales[s], i));
-#pragma unroll
-                for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, x.part[s][t][i], acc[t], 0, 0, 0);
-            }
-        // under the sums and stores of this one
-        if (LONG && turn + 1 == turns && phase + 1 < phases) load(tile_of(0) + group, phase + 1, ahead);
-        else load(tile_of(turn + 1) + group, phase, ahead);
-        float (*mine)[TT][256] = sums[turn & 1];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) *reinterpret_cast<v4f32*>(&mine[wave][t][(lane & 15) * 16 + 4 * q]) = acc[t];
+        if (phase) __syncthreads();  // the last turn's sums are read
+        W4Rows<S, TT> x;
+        x.load(a, row0, rows, phase * (W * S) + slice * S, shared + wave * kTurnBytes);
         __syncthreads();
-        const __amdgpu_buffer_rsrc_t y = w4_run_of(static_cast<OUT*>(a.y) + row0 * a.y_pitch + long(tile) * 16, kRunMost);
-        const long left = a.w.n - long(tile) * 16;
-        for (int i = wave * 64 + lane; i < groups * TT * 256; i += threads) {
-            const int g = i / (TT * 256), t = i / 256 % TT, cell = i % 256, r = 16 * t + cell / 16, c = 16 * g + cell % 16;
-            float s = 0.0f;
+        for (int turn = 0; turn < turns; ++turn) {  // the same for every wave
+            const int tile = tile_of(turn);
+            v4f32 acc[TT];
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float part = mine[g * slices + (w < slices ? w : 0)][t][cell];
-                s += w < slices ? part : 0.0f;
-            }
-            if (LONG) {
-                if (phase) s += kept[turn][i];
-                kept[turn][i] = s;
-                if (phase + 1 < phases) continue;
-            }
-            const int at = (r * int(a.y_pitch) + c) * int(sizeof(OUT));
-            if (r < rows && c < left) {
-                if constexpr (sizeof(OUT) == 2) __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bf16_rne_nan(s)), y, at, 0, 0);
-                else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s), y, at, 0, 0);
+            for (int t = 0; t < TT; ++t) acc[t] = v4f32{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v8bf wide = w4_widen(ahead.codes[s][i], w4_scale(ahead.scales[s], i));
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wide, x.part[s][t][i], acc[t], 0, 0, 0);
+                }
+            // under the sums and stores of this one
+            if (LONG && turn + 1 == turns && phase + 1 < phases) load(tile_of(0) + group, phase + 1, ahead);
+            else load(tile_of(turn + 1) + group, phase, ahead);
+            float (*mine)[TT][256] = sums[turn & 1];
+#pragma unroll
+            for (int t = 0; t < TT; ++t) *reinterpret_cast<v4f32*>(&mine[wave][t][(lane & 15) * 16 + 4 * q]) = acc[t];
+            __syncthreads();
+            const __amdgpu_buffer_rsrc_t y = w4_run_of(static_cast<OUT*>(a.y) + row0 * a.y_pitch + long(tile) * 16, kRunMost);
+            const long left = a.w.n - long(tile) * 16;
+            for (int i = wave * 64 + lane; i < groups * TT * 256; i += threads) {
+                const int g = i / (TT * 256), t = i / 256 % TT, cell = i % 256, r = 16 * t + cell / 16, c = 16 * g + cell % 16;
+                float s = 0.0f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float part = mine[g * slices + (w < slices ? w : 0)][t][cell];
+                    s += w < slices ? part : 0.0f;
+                }
+                if (LONG) {
+                    if (phase) s += kept[turn][i];
+                    kept[turn][i] = s;
+                    if (phase + 1 < phases) continue;
+                }
+                const int at = (r * int(a.y_pitch) + c) * int(sizeof(OUT));
+                if (r < rows && c < left) {
+                    if constexpr (sizeof(OUT) == 2) __builtin_amdgcn_raw_buffer_store_b16(uint16_t(bf16_rne_nan(s)), y, at, 0, 0);
+                    else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s), y, at, 0, 0);
+                }
             }
         }
-    }
     }
 }
 
