@@ -558,6 +558,62 @@ def test_logprobs_without_optional_outputs_and_twice_the_same():
     assert np.array_equal(first[0].reshape(3, 4), R.logprobs(x, np.zeros((3, 0), int), 4, 1.0)[2])
 
 
+# ---- far apart ----------------------------------------------------------------------------------------------
+
+def put(at, a):
+    a = np.ascontiguousarray(a)
+    assert b1.load().m26s_b1_copy_to_device(at, a.ctypes.data, a.nbytes) == 0
+
+
+def take(at, shape, dtype):
+    a = np.empty(shape, dtype)
+    assert b1.load().m26s_b1_copy_to_host(a.ctypes.data, at, a.nbytes) == 0
+    return a
+
+
+def test_rows_further_apart_than_32_bits_reach():
+    """Pitches that put a row past 2^32 bytes from the first; what lies between is not touched."""
+    far = b1.DeviceBuffer(5 << 30)
+    rng = np.random.default_rng(12)
+    for vocab, half in ((1000, True), (20001, True), (20001, False)):
+        size, pitch = x_size(half), ((1 << 32) // x_size(half)) + 5
+        x = some_logits(rng, 2, vocab, half)
+        for r in range(2):
+            put(far.ptr + r * pitch * size, R.bf16(x[r])[0] if half else x[r])
+        given = np.array([[3, 3, vocab - 1], [vocab // 2, -1, 0]], np.int32)
+        gd, gl, en, ti, tl = dev(given), room(24), room(8), room(40), room(40)
+        need = coord.token_logprobs_workspace(2, vocab, 5)
+        ws = room(need)
+        coord.token_logprobs(far.ptr, half, 2, vocab, pitch, gd.ptr, 3, gl.ptr, en.ptr, 5, ti.ptr, tl.ptr, ws.ptr, need)
+        check_logprobs((gl.to_host(np.float32).reshape(2, 3), en.to_host(np.float32), ti.to_host(np.int32).reshape(2, 5),
+                        tl.to_host(np.float32).reshape(2, 5)), x, given, 5, 1.0)
+    # the join in place, a plane's rows and the normed rows between those of h
+    cols = 96
+    h, planes, pre, _, _ = join_inputs(2, cols, 1, False, "none", 2)
+    hp, pp = (1 << 30) + 64, (1 << 31) + 64
+    for r in range(2):
+        put(far.ptr + r * hp * 4, h[r])
+        put(far.ptr + 4096 + r * pp * 2, planes[0][0][r])
+    w = dev(pre)
+    plan = coord.Join(cols, w.ptr, scale=0.5, eps=1e-5, plane_pitch=pp, h_pitch=hp, norm_pitch=pp)
+    plan(2, far.ptr, [far.ptr + 4096], far.ptr, norm=far.ptr + 8192)
+    got = {"h": np.stack([take(far.ptr + r * hp * 4, cols, np.float32) for r in range(2)]),
+           "norm": np.stack([take(far.ptr + 8192 + r * pp * 2, cols, np.uint16) for r in range(2)])}
+    check_join(got, h, planes, pre, None, None, 0.5, 1e-5)
+    # products: the largest pitches of x and y
+    rows, n, k, pitch = 70, 40, 96, 1 << 24
+    rng, payload, scales = w4_inputs(n, k, 3)
+    weights = weights_of(payload, scales)
+    bits, value = R.bf16(rng.standard_normal((rows, k)).astype(np.float32))
+    for r in range(rows):
+        put(far.ptr + 4096 + r * pitch * 2, bits[r])
+        put(far.ptr + r * pitch * 4 + n * 4, np.full(4, 7.0, np.float32))
+    weights.matvec(far.ptr + 4096, rows, far.ptr, x_pitch=pitch, y_pitch=pitch)
+    y = np.stack([take(far.ptr + r * pitch * 4, n + 4, np.float32) for r in range(rows)])
+    want, tol = R.w4_product(value, R.w4_weights(payload, scales))
+    assert np.all(np.abs(y[:, :n] - want) <= tol) and (y[:, n:] == 7.0).all()
+
+
 # ---- together ------------------------------------------------------------------------------------------------
 
 def test_a_step_from_the_ranks_rows_to_the_answer():
