@@ -137,11 +137,13 @@ int launch_resident(const W4Args& a, int workgroups, int share, hipStream_t st) 
 //    against 9.7 the other way. Eight waves, a step at a time: sixteen lose where tiles meet on a compute unit (626 x 17 of wire
 //    rows 9.4 against 7.0), and so do two steps on their way (6.8 against 6.3), which gain on long k (125 x 128, 16 rows 9.8
 //    against 11.4; 256 x 64, 1 row 6.3 against 7.1).
-//  * otherwise resident rows, one workgroup per compute unit over all row runs, so that each loads its rows once. Sixteen waves
-//    hold sixteen rows up to 64 steps (8192 tiles x 32 steps: 48.3 us with sixteen waves of two steps, 50.1 with eight of
-//    four) and 32 rows up to 32 (1024 x 32, 64 rows: 17.8 against 22.3 with 16 a run); up to sixteen steps eight waves do, twice as
-//    many workgroups up to eight steps (2048 x 8: 7.8 against 8.9). Past 64 steps in phases, again 32 rows a run (1875 x
-//    80, 64 rows: 88 against 110), but from 33 to 64 sixteen, which need none (2000 x 64, 64 rows: 56 against 68).
+//  * otherwise resident rows, as many workgroups over all row runs as fit on the compute units at once, so that each loads its
+//    rows once. Sixteen waves hold sixteen rows up to 64 steps (8192 tiles x 32 steps: 48.3 us with sixteen waves of two steps, 50.1
+//    with eight of four) and 32 rows up to 32 (1024 x 32, 64 rows: 17.8 against 22.3 with 16 a run). Up to 24 steps a workgroup of
+//    sixteen rows has twelve waves at most, and two of them fit (3750 x 18: 17.4 against 20.4 with one; of 32 rows the registers
+//    do not allow it, 64 rows 45 against 39); up to sixteen steps two of eight waves (8192 x 16, 16 rows 27.6 against 37, 64 rows
+//    68 against 76), up to eight steps four (8192 x 8: 17.4 against 21.5 with two). Past 64 steps in phases, again 32 rows a
+//    run (1875 x 80, 64 rows: 88 against 110), but from 33 to 64 sixteen, which need none (2000 x 64, 64 rows: 56 against 68).
 int launch_w4(const W4Args& a, hipStream_t st) {
     const int steps = a.w.steps, runs16 = (a.rows + 15) / 16;
     if (long(a.w.tiles) * runs16 <= 768) {
@@ -154,14 +156,14 @@ int launch_w4(const W4Args& a, hipStream_t st) {
     const int runs = a.rows > 16 && (steps <= 32 || steps > 64) ? (a.rows + 31) / 32 : runs16, share = (a.rows + runs - 1) / runs;
     const int workgroups = runs < 256 ? 256 / runs : 1;
     if (share > 16) {
-        if (steps <= 8) return launch_resident<2, 1, 8>(a, 2 * workgroups, share, st);
-        if (steps <= 16) return launch_resident<2, 2, 8>(a, workgroups, share, st);
+        if (steps <= 8) return launch_resident<2, 1, 8>(a, 4 * workgroups, share, st);
+        if (steps <= 16) return launch_resident<2, 2, 8>(a, 2 * workgroups, share, st);
         if (steps <= 32) return launch_resident<2, 2, 16>(a, workgroups, share, st);
         return launch_resident<2, 2, 16, true>(a, workgroups, share, st);
     }
-    if (steps <= 8) return launch_resident<1, 1, 8>(a, 2 * workgroups, share, st);
-    if (steps <= 16) return launch_resident<1, 2, 8>(a, workgroups, share, st);
-    if (steps <= 32) return launch_resident<1, 2, 16>(a, workgroups, share, st);
+    if (steps <= 8) return launch_resident<1, 1, 8>(a, 4 * workgroups, share, st);
+    if (steps <= 16) return launch_resident<1, 2, 8>(a, 2 * workgroups, share, st);
+    if (steps <= 32) return launch_resident<1, 2, 16>(a, steps <= 24 ? 2 * workgroups : workgroups, share, st);
     if (steps <= 48) return launch_resident<1, 3, 16>(a, workgroups, share, st);
     if (steps <= 64) return launch_resident<1, 4, 16>(a, workgroups, share, st);
     const int threes = (steps + 47) / 48 * 3, fours = (steps + 63) / 64 * 4;  // steps a wave goes through
