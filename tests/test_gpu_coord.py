@@ -243,7 +243,7 @@ SHAPES = [(1, 1, 32), (1, 16, 64), (3, 17, 96), (16, 256, 4096), (17, 100, 128),
           (1, 4096, 4096), (2, 5, 16384), (48, 4099, 608), (16, 33000, 256),
           # every form of the rule on sizes: steps of 128 up to 8, 16, 24, 32, 48, 64 and more, in runs of 16 and 32 rows, tiles past one turn
           (3, 13000, 1056), (16, 12500, 2080), (9, 12400, 3200), (7, 12400, 4128), (5, 12330, 6176), (2, 12330, 8224), (33, 8200, 96), (29, 13000, 1056),
-          (64, 8200, 2080), (50, 4200, 3200), (64, 4200, 4128), (300, 200, 640), (2, 40, 16416), (33, 3104, 16416), (1, 1, 64), (3, 7, 96)]
+          (64, 8200, 2080), (50, 4200, 3200), (64, 4200, 4128), (300, 200, 640), (2, 40, 16416), (33, 3104, 16416), (1, 1, 64), (3, 7, 96), (16, 16500, 2080), (3, 16500, 1056)]
 
 
 @pytest.mark.parametrize("rows,n,k", SHAPES)
