@@ -301,7 +301,7 @@ int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_
 }
 
 constexpr int kVocabMost = 1 << 30;           // ids past a row's end, up to a chunk of every part, still fit
-constexpr float kScaleMost = float(1 << 20);  // a scaled logit that is measured from a rounded maximum stays finite
+constexpr float kScaleMost = float(1 << 20);  // a temperature of a millionth: scale * log2 e and ordinary logits times it stay finite
 
 size_t m26c_token_logprobs_workspace(int rows, int vocab, int top) {
     if (rows <= 0 || vocab <= 0 || vocab > kVocabMost || top < 0 || top > kTopMost) return 0;
@@ -312,8 +312,8 @@ size_t m26c_token_logprobs_workspace(int rows, int vocab, int top) {
 int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int vocab, float scale, const int* given, int n_given,
                         float* given_logprob, float* entropy, int top, int* top_ids, float* top_logprob, void* workspace,
                         size_t workspace_bytes, void* stream) {
-    if (rows < 0 || vocab <= 0 || vocab > kVocabMost || n_given < 0 || top < 0 || top > kTopMost || top > vocab || !(scale > 0.0f && scale <= kScaleMost) ||
-        pitch < vocab)
+    if (rows < 0 || vocab <= 0 || vocab > kVocabMost || n_given < 0 || n_given > kVocabMost || top < 0 || top > kTopMost || top > vocab ||
+        !(scale > 0.0f && scale <= kScaleMost) || pitch < vocab)
         return 1;
     if (rows == 0) return 0;
     if (!logits || !on(logits, bf16 ? 2 : 4) || (n_given && (!given || !given_logprob || !on(given, 4) || !on(given_logprob, 4))) || !on(entropy, 4) ||

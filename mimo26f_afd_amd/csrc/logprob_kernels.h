@@ -78,19 +78,31 @@ __device__ __forceinline__ float wave_max(float v) {  // as wave_sum
 
 // Running sums of 2^(v c - r), c = scale * log2 e, and of that times its exponent, relative to r = m c rounded to FP32, m the
 // largest value so far: the exponent is then one fused multiply-add, rounded once, and r, the same number everywhere, comes
-// out again at the end. Values so large that m c may pass FP32's range (masks of the type's lowest value in a row of nothing
-// else) are measured from m itself, (v - m) c.
+// out again at the end. From 2^24 on that rounding is more than one, up to any size (masks of -1e9, or of the type's lowest
+// value, in a row of nothing else): such values are `far`, and measured from m itself, (v - m) c.
 struct SoftmaxSums {
     float m = -INFINITY, z = 0.0f, s = 0.0f;
 
-    __device__ __forceinline__ static bool far(float m) { return fabsf(m) > 1e30f && m != -INFINITY; }
+    __device__ __forceinline__ static bool far(float m, float c) { return fabsf(m * c) > 16777216.0f && m != -INFINITY; }
     __device__ __forceinline__ static float distance(float v, float m, float c) {
-        return far(m) ? (v - m) * c : __builtin_fmaf(v, c, m == -INFINITY ? 0.0f : -(m * c));
+        return far(m, c) ? (v - m) * c : __builtin_fmaf(v, c, m == -INFINITY ? 0.0f : -(m * c));
     }
     // The sums relative to the maximum `to` (>= m). Without a number so far z and s are 0, or NaN.
     __device__ __forceinline__ SoftmaxSums at(float to, float c) const {
-        const float d = m == to || m == -INFINITY ? 0.0f : far(m) || far(to) ? (m - to) * c : m * c - to * c, f = __builtin_amdgcn_exp2f(d);
-        return SoftmaxSums{to, f * z, f * (s + (d == -INFINITY ? 0.0f : d * z))};
+        const bool here = far(m, c), there = far(to, c);
+        const float between = here == there ? (here ? (m - to) * c : m * c - to * c)
+                                            : here ? __builtin_fmaf(m, c, -(to * c)) : -__builtin_fmaf(to, c, -(m * c));
+        return moved(to, m == to || m == -INFINITY ? 0.0f : between);
+    }
+    // The same where all sums are relative to a rounded r, whatever its size.
+    __device__ __forceinline__ SoftmaxSums at_rounded(float to, float c) const {
+        return moved(to, m == to || m == -INFINITY ? 0.0f : m * c - to * c);
+    }
+    // What is left far behind counts nothing, even if a rounded r had made it infinite; NaN stays.
+    __device__ __forceinline__ SoftmaxSums moved(float to, float d) const {
+        if (d < -256.0f) return SoftmaxSums{to, z != z ? z : 0.0f, z != z ? z : 0.0f};
+        const float f = __builtin_amdgcn_exp2f(d);
+        return SoftmaxSums{to, f * z, f * (s + d * z)};
     }
     __device__ __forceinline__ void join(const SoftmaxSums& o, float c) {
         const float to = fmaxf(m, o.m);
@@ -282,13 +294,15 @@ struct RowPart {
     }
     // The whole chunks, in pairs, with the next pair on its way. Past the end the last chunk is asked for again: a load under a
     // condition would make the compiler wait for all of them. One copy of the work on a chunk: unrolled over a ring of four it
-    // was 45 KB of code, which a short call fetches as it goes.
+    // was 45 KB of code, which a short call fetches as it goes. True if the sums are not to be trusted: a NaN, or nothing but far values.
     template <typename LIST>
-    __device__ __forceinline__ void quickly(const LogprobArgs& a, SoftmaxSums& sum, LIST& list, float c) const {
+    __device__ __forceinline__ bool quickly(const LogprobArgs& a, SoftmaxSums& sum, LIST& list, float c) const {
         const int lane = threadIdx.x & 63, final_chunk = part + (chunks - 1 - part) / parts * parts;
         auto ask = [&](int chunk) { return load(chunk < final_chunk ? chunk : final_chunk); };
         Raw first = ask(part), second = ask(part + parts);
-        float r = sum.m == -INFINITY ? 0.0f : -(sum.m * c);
+        const SoftmaxSums ahead = sum;  // of the boundary
+        sum = SoftmaxSums{};
+        float r = 0.0f;
         for (int chunk = part; chunk <= final_chunk;) {
             const Raw third = ask(chunk + 2 * parts), fourth = ask(chunk + 3 * parts);
 #pragma nounroll
@@ -299,7 +313,7 @@ struct RowPart {
 #pragma unroll
                 for (int j = 1; j < 8; ++j) most = fmaxf(most, v[j]);
                 if (__any(most > sum.m)) {
-                    sum = sum.at(fmaxf(most, sum.m), c);
+                    sum = sum.at_rounded(fmaxf(most, sum.m), c);
                     r = sum.m == -INFINITY ? 0.0f : -(sum.m * c);
                 }
 #pragma unroll
@@ -311,17 +325,23 @@ struct RowPart {
             first = third;
             second = fourth;
         }
+        // Lanes that saw nothing but masks: their far maximum does not matter beside the wave's.
+        const float largest = wave_max(sum.m);
+        if (SoftmaxSums::far(sum.m, c) && !SoftmaxSums::far(largest, c)) sum = sum.at_rounded(largest, c);
+        const bool lost = __any(sum.z != sum.z || SoftmaxSums::far(sum.m, c));
+        sum.join(ahead, c);
+        return lost;
     }
 
     template <typename LIST>
     __device__ __forceinline__ void walk(const LogprobArgs& a, SoftmaxSums& sum, LIST& list) const {
         const int lane = threadIdx.x & 63, done = head + chunks * kChunk;
         const float c = a.scale * 1.44269504088896341f;
-        // A part that turns out to hold a NaN or values past what the quick form measures is gone through once more, slowly.
-        for (bool careful = false;; careful = true) {
+        // A part whose whole chunks turn out to hold a NaN, or nothing but far values, is gone through once more, slowly.
+        for (bool careful = false, lost = false;; careful = true) {
             for (int phase = 0; phase < 3; ++phase) {  // ahead of the boundary; whole chunks; what is left behind them
                 if (phase == 1 && !careful) {
-                    if (part < chunks) quickly(a, sum, list, c);
+                    if (part < chunks) lost = quickly(a, sum, list, c);
                     continue;
                 }
                 const bool mine = phase == 0 ? part == 0 : phase == 1 || part == parts - 1;
@@ -329,7 +349,7 @@ struct RowPart {
                 for (int id = phase == 0 ? 0 : phase == 1 ? head + part * kChunk : done; mine && id < stop; id += parts * kChunk)
                     slowly(a, sum, list, id + lane * 8, stop, c);
             }
-            if (careful || !__any(sum.z != sum.z || SoftmaxSums::far(sum.m))) break;
+            if (careful || !lost) break;
             sum = SoftmaxSums{};
             list.key = kNoKey;
             list.threshold = -INFINITY;
@@ -372,7 +392,7 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
     constexpr float kLn2 = 0.69314718055994531f;
     const bool empty = sum.m == -INFINITY && sum.z == 0.0f;
     // Z is relative to 2^r, r = m c rounded: what r is short of m c is exactly a fused product
-    const float ln_z = kLn2 * (SoftmaxSums::far(sum.m) || sum.m == -INFINITY ? log_z : log_z - __builtin_fmaf(sum.m, c, -(sum.m * c)));
+    const float ln_z = kLn2 * (SoftmaxSums::far(sum.m, c) || sum.m == -INFINITY ? log_z : log_z - __builtin_fmaf(sum.m, c, -(sum.m * c)));
     auto logprob = [&](float v) { return (v - sum.m) * a.scale - ln_z; };
     if (tid == 0 && a.entropy) a.entropy[row] = empty ? 0.0f : kLn2 * (log_z - sum.s / sum.z);
     for (int i = tid; i < a.n_given; i += THREADS) {

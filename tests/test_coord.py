@@ -74,7 +74,7 @@ def logprob_call(logits=P, bf16=False, rows=2, vocab=100, pitch=100, given=P, n_
                                     dict(given=None), dict(given_logprob=None), dict(n_given=-1), dict(given=P + 2), dict(entropy=P + 1), dict(top=-1),
                                     dict(top=33), dict(top=4, vocab=3), dict(top_ids=None), dict(top_logprob=None), dict(scale=0.0), dict(scale=-1.0),
                                     dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=2.0 ** 20 * (1 + 2.0 ** -20)),
-                                    dict(vocab=(1 << 30) + 1, pitch=1 << 31), dict(rows=1, vocab=131072, pitch=131072, workspace=None),
+                                    dict(vocab=(1 << 30) + 1, pitch=1 << 31), dict(n_given=(1 << 30) + 1), dict(rows=1, vocab=131072, pitch=131072, workspace=None),
                                     dict(rows=1, vocab=131072, pitch=131072, workspace=P + 8),
                                     dict(rows=1, vocab=131072, pitch=131072, workspace_bytes=16)])
 def test_logprobs_refuse(change):

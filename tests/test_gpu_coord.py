@@ -427,9 +427,13 @@ def x_size(half):
 
 
 def check_logprobs(got, logits, given, top, scale):
-    gl, en, ids, lp = got
     with np.errstate(all="ignore"):
-        wg, wh, wi, wl, tg, th, tt = R.logprobs(logits, given, top, scale)
+        check_logprobs_against(got, R.logprobs(logits, given, top, scale))
+
+
+def check_logprobs_against(got, want):
+    gl, en, ids, lp = got
+    wg, wh, wi, wl, tg, th, tt = want
     assert np.array_equal(ids, wi)
 
     def near(a, b, tol):
@@ -519,6 +523,37 @@ def test_logprobs_of_rows_that_are_hard_to_select_from(half, vocab):
         check_logprobs(run_logprobs(np.ascontiguousarray(x), given, top, 1.0, half), x.astype(np.float64), given, top, 1.0)
         single = np.concatenate([run_logprobs(x[r:r + 1], given[r:r + 1], top, 1.0, half)[2] for r in range(len(rows))])
         assert np.array_equal(single, run_logprobs(x, given, top, 1.0, half)[2])   # however a row is cut, the same ids
+
+
+def rows_of_large_numbers(vocab, half):
+    """Logits so large that the rounding of scaled ones is more than the differences that matter, and masks like them."""
+    rng = np.random.default_rng(vocab + 1)
+    rows = [np.full(vocab, v) for v in (-1e9, -1e10, -3e20, 1e10, 9e29, 2e7)]                   # equal ones: the entropy is ln vocab
+    for low in (-1e9, -1e10, -3e20, -1e38):                                                     # masks: a few tokens, one late token, half of them
+        for kept in (np.arange(3, vocab, 997), np.array([vocab - 2]), np.arange(0, vocab, 2)):
+            row = np.full(vocab, low)
+            row[kept] = rng.standard_normal(kept.size) * 3
+            rows.append(row)
+    for base, step in ((11629080.0, 1.0), (-11629080.0, 1.0), (5e8, 32.0), (-5e8, 32.0)):       # 2^24 in units of log2, and past it
+        rows.append(base + step * rng.integers(-60, 1, vocab))
+        rows.append(base + step * np.sort(rng.integers(-9, 9, vocab)))
+    x = np.stack(rows).astype(np.float32)
+    return R.bf16(x)[1] if half else x
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("vocab,copies,top,scale", [(700, 1, 8, 1.0), (5003, 1, 20, 0.7), (5003, 80, 8, 1.0), (20011, 1, 8, 1.25), (20011, 60, 5, 1.0),
+                                                    (100003, 4, 8, 1.0), (5003, 1, 4, 2.0 ** 20), (5003, 80, 4, 2.0 ** -20)])
+def test_logprobs_of_large_numbers(half, vocab, copies, top, scale):
+    x = rows_of_large_numbers(vocab, half)
+    n = len(x)
+    given = np.stack([[vocab // 3, 0, vocab - 2]] * n)
+    got = run_logprobs(np.tile(x, (copies, 1)), np.tile(given, (copies, 1)), top, scale, half, shift=3)
+    with np.errstate(over="ignore"):
+        gl, en, ids, lp = (g.reshape(copies, n, -1) for g in got)
+        for i in (0, copies - 1):                                                               # a log probability past FP32 is -infinity
+            want = R.logprobs(x, given, top, scale)
+            check_logprobs_against((gl[i], en[i, :, 0], ids[i], lp[i]), tuple(w.astype(np.float32) if k in (0, 3) else w for k, w in enumerate(want)))
 
 
 @pytest.mark.parametrize("half", [False, True])
