@@ -27,7 +27,8 @@ extern "C" {
  *   h' = h + scale * gate * z                           FP32
  *   n  = h' * pre_weight / sqrt(mean(h'^2) + eps)
  * Outputs: h' (FP32), and n as BF16 (nearest even) and / or as wire rows: E4M3 codes with one UE8M0 byte per 32 values by
- * the rule of m26c_quantize_hidden, taken from the FP32 n. Sums are FP32. A NaN or an infinity of a row stays in its row.
+ * the rule of m26c_quantize_hidden, taken from the FP32 n. Sums are FP32 (a row whose sum of squares passes FP32's range is
+ * normed to zero). A NaN or an infinity of a row stays in its row.
  * The plan holds what a program keeps from call to call. Pitches count elements (bytes for payload and scales); rows of
  * `cols` values, 1 <= cols <= 16384, a multiple of 32 for wire rows. Any alignment of the element type is accepted. */
 typedef struct m26c_join {

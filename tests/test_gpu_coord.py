@@ -366,6 +366,18 @@ def test_w4_bad_values_of_x_stay_in_their_row():
     assert np.all(np.abs(got[[0, 3]] - want) <= tol) and np.isnan(got[[1, 2]]).all()
 
 
+@pytest.mark.parametrize("rows,n,k", [(3, 40, 160), (20, 16400, 256)])
+def test_w4_subnormal_values_of_x_count(rows, n, k):
+    """BF16 values below 2^-126 under weights large enough to make ordinary products of them."""
+    rng, payload, _ = w4_inputs(n, k, rows)
+    weights_scales = np.full((n, k // 32), 252, np.uint8)
+    weights = weights_of(payload, weights_scales)
+    bits = (rng.integers(0, 128, (rows, k)) | rng.integers(0, 2, (rows, k)) << 15).astype(np.uint16)
+    want, tol = R.w4_product(R.widen(bits), R.w4_weights(payload, weights_scales))
+    got = run_w4(weights, bits, rows)
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
 def test_w4_wire_rows_at_the_ends_of_the_scale_range():
     rng, payload, scales = w4_inputs(40, 128, 6, 126, 129)
     weights = weights_of(payload, scales)
