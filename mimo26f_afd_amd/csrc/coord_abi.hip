@@ -135,7 +135,8 @@ int launch_resident(const W4Args& a, int workgroups, int share, hipStream_t st) 
 //  * few tiles and rows: a workgroup per tile, rows streamed with the weights, as long as there is one per compute unit at most (256
 //    tiles x 32 steps, 1 row 3.9 against 4.9 with resident rows; 157 x 128 9.8 against 12.9) or up to four with little to do each
 //    (813 x 8, 16 rows 4.5 against 5.3; 626 x 17, 5 wire rows 6.5 against 7.8; 313 x 64 11.0 against 9.5 and 563 x 32 of
-//    wire rows 10.9 against 8.9 the other way). Eight waves, a step at a time: sixteen lose where tiles meet on a compute
+//    wire rows 10.9 against 8.9 the other way; against phases longer, 468 x 68 10.9 against 21.4, 750 x 68 16.2 against 19.7, 750 x
+//    128 37 against 25 the other way). Eight waves, a step at a time: sixteen lose where tiles meet on a compute
 //    unit (626 x 17 of wire rows 9.4 against 7.0), and so do two steps on their way (6.8 against 6.3), which gain on long k
 //    (125 x 128, 16 rows 9.8 against 11.4; 256 x 64, 1 row 6.3 against 7.1).
 //  * otherwise resident rows, as many workgroups over all row runs as fit on the compute units at once, so that each loads its
@@ -148,7 +149,7 @@ int launch_resident(const W4Args& a, int workgroups, int share, hipStream_t st) 
 int launch_w4(const W4Args& a, hipStream_t st) {
     const int steps = a.w.steps, runs16 = (a.rows + 15) / 16;
     const long cells = long(a.w.tiles) * runs16;
-    if (cells <= 256 || (cells <= 1024 && cells * steps <= 17000)) {
+    if (cells <= 256 || (cells <= 1024 && cells * steps <= (steps > 64 ? 72000 : 17000))) {
         const int share = (a.rows + runs16 - 1) / runs16;
         const dim3 grid(over_xcds(a.w.tiles, runs16), unsigned(runs16));
         if (steps >= 64) w4_streamed_kernel<8, 2><<<grid, 512, 0, st>>>(a, share);
