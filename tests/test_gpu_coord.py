@@ -366,6 +366,23 @@ def test_w4_bad_values_of_x_stay_in_their_row():
     assert np.all(np.abs(got[[0, 3]] - want) <= tol) and np.isnan(got[[1, 2]]).all()
 
 
+@pytest.mark.parametrize("form", ["bf16", "fp8"])
+def test_w4_more_rows_than_a_launch_takes(form):
+    rows, n, k = (1 << 19) + 21, 3, 32
+    rng, payload, scales = w4_inputs(n, k, 9)
+    weights = weights_of(payload, scales)
+    x = rng.standard_normal((rows, k)).astype(np.float32)
+    if form == "bf16":
+        bits, value = R.bf16(x)
+        got = run_w4(weights, bits, rows, y_pad=1)
+    else:
+        wire = O.q0_quantize(x)
+        value = R.wire_values(*wire)
+        got = run_w4(weights, None, rows, fp8=wire, y_pad=1)
+    want, tol = R.w4_product(value, R.w4_weights(payload, scales))
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
 @pytest.mark.parametrize("rows,n,k", [(3, 40, 160), (20, 16400, 256)])
 def test_w4_subnormal_values_of_x_count(rows, n, k):
     """BF16 values below 2^-126 under weights large enough to make ordinary products of them."""
