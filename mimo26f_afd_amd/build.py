@@ -15,7 +15,7 @@ LIB = os.path.join(HERE, "lib", "libm26s_b1.so")
 PROBE_LIB = os.path.join(HERE, "lib", "libm26_probe.so")
 SOURCES = ["csrc/b1_abi.hip", "csrc/glue_abi.hip", "csrc/coord_abi.hip", "csrc/frame_abi.hip"]
 DEPENDS = ["csrc/b1_kernels.h", "csrc/b1_tile.h", "csrc/b1_conform.h", "csrc/b1_layout.h", "csrc/glue_kernels.h",
-           "csrc/q0_codec.h", "csrc/join_kernels.h", "csrc/w4_kernels.h", "csrc/logprob_kernels.h",
+           "csrc/q0_codec.h", "csrc/wave_fence.h", "csrc/join_kernels.h", "csrc/w4_kernels.h", "csrc/logprob_kernels.h",
            "../include/m26s_b1.h", "../include/m26c_glue.h", "../include/m26c_coord.h", "../include/m26w_frame.h"]
 PROBE_SOURCES = ["csrc/probe_abi.hip"]
 PROBE_DEPENDS = ["../include/m26_probe.h"]

@@ -27,6 +27,7 @@
 #include <stdint.h>
 #include <type_traits>
 #include "join_kernels.h"
+#include "wave_fence.h"
 
 namespace m26g {
 
@@ -141,12 +142,6 @@ __device__ __forceinline__ uint32_t reached_by(const uint32_t (&v)[N], int top) 
         cut = n3 >= top ? k3 : n2 >= top ? k2 : n1 >= top ? k1 : cut;
     }
     return cut;
-}
-
-// Orders what other lanes of this wave have written to LDS before what this lane reads next.
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
 }
 
 // The next number below v; below zero that is the smallest negative one.

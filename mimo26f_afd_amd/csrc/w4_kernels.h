@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "q0_codec.h"
+#include "wave_fence.h"
 
 namespace m26g {
 
@@ -105,7 +106,8 @@ constexpr int kStreamed = 2;  // non-temporal: a weight is used once
 // A lane's share of STEPS k-steps of TT * 16 rows of x, as MFMA operands. The operand order asks for 64 bytes of each of
 // sixteen rows at a time, which a compute unit's memory path serves at 16 bytes a cycle; four rows of 256 bytes come at
 // 40 to 52. So a wave loads whole steps of rows, 256 bytes (128 of wire rows) each, and turns them round in a corner of LDS
-// of its own. All loads are issued before the first is looked at; what is past k or past the last row is asked for outside the
+// of its own, with a fence between the lanes' writes and the other lanes' reads and one behind the reads, ahead of the next step's
+// writes. All loads are issued before the first is looked at; what is past k or past the last row is asked for outside the
 // buffer, which moves nothing and gives zero. (Past k the weights are zero and x has to be a number.)
 constexpr int kTurnRow = 256 + 16, kTurnBytes = 16 * kTurnRow;  // a row's step in LDS, padded so that the rows of a column start in different banks
 template <int STEPS, int TT>
@@ -147,6 +149,7 @@ struct W4Rows {
                 for (int t = 0; t < TT; ++t) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) *reinterpret_cast<v2u32*>(corner + (4 * i + q) * kTurnRow + c * 8) = raw[s][t][i];
+                    wave_fence();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const v2u32 code = *reinterpret_cast<const v2u32*>(corner + c * kTurnRow + i * 32 + q * 8);
@@ -161,6 +164,7 @@ struct W4Rows {
                         for (int j = 0; j < 4; ++j) u.dword[j] = byte == 255u ? 0x7fc07fc0u : u.dword[j];  // 255 is not a number
                         part[s][t][i] = u.all;
                     }
+                    wave_fence();
                 }
         } else {
             const __amdgpu_buffer_rsrc_t x = w4_run_of(a.x + row0 * a.x_pitch, kRunMost);
@@ -181,8 +185,10 @@ struct W4Rows {
                 for (int t = 0; t < TT; ++t) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) *reinterpret_cast<v4u32*>(corner + (4 * i + q) * kTurnRow + c * 16) = raw[s][t][i];
+                    wave_fence();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) part[s][t][i] = *reinterpret_cast<const v8bf*>(corner + c * kTurnRow + i * 64 + q * 16);
+                    wave_fence();
                 }
         }
     }
