@@ -69,9 +69,9 @@ void m26c_w4_free(m26c_w4* w);
 int m26c_w4_matvec(const m26c_w4* w, const uint16_t* x, long x_pitch, int rows, void* y, int y_bf16, long y_pitch, void* stream);
 
 /* The same on wire rows: E4M3 codes and one UE8M0 byte per 32 values, at their own pitches in bytes (request-frame rows are
- * read in place); payload 8-byte aligned, its pitch a multiple of 8. Codes are taken exactly for scale bytes 10..246. Byte
- * 255 and NaN codes make their row NaN; above 246 a code past BF16's range counts as infinite; below 10 a code stands
- * for less than 2^-108 and may lose its low bits. */
+ * read in place); payload 8-byte aligned, its pitch a multiple of 8. Codes are taken exactly for scale bytes 3..246. Byte
+ * 255 and NaN codes make their row NaN; above 246 a code past BF16's range counts as infinite; for bytes 0..2 a code's value
+ * is rounded to a multiple of 2^-133 (nearest even). */
 int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_pitch, const uint8_t* scales, size_t scales_pitch,
                        int rows, void* y, int y_bf16, long y_pitch, void* stream);
 

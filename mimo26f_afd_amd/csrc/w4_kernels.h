@@ -154,7 +154,9 @@ struct W4Rows {
                     for (int i = 0; i < 4; ++i) {
                         const v2u32 code = *reinterpret_cast<const v2u32*>(corner + c * kTurnRow + i * 32 + q * 8);
                         const uint32_t byte = scale[s][t] >> (8 * i) & 0xffu;
-                        const float f = __uint_as_float((byte ? byte : 1u) << 23);  // byte 0 marks a block of zeros
+                        // The conversion reads the exponent field alone: byte 0 is 2^-127, which blocks of the smallest values carry. Codes are
+                        // exact up to byte 246; under bytes 0..2 they are rounded to multiples of 2^-133, BF16's smallest step.
+                        const float f = __uint_as_float(byte << 23);
                         union { v2bf pair[4]; v8bf all; uint32_t dword[4]; } u;
                         u.pair[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code.x, f, false);
                         u.pair[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code.x, f, true);

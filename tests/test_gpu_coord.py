@@ -409,6 +409,60 @@ def test_w4_wire_rows_at_the_ends_of_the_scale_range():
     assert (run_w4(weights, None, 8, fp8=(zero, np.zeros((8, 4), np.uint8))) == 0).all()
 
 
+def on_the_grid(x):
+    """What the products take wire values as: multiples of 2^-133, the step of BF16's smallest numbers, nearest even. It takes a
+    scale byte below 3 for a code to have bits under that."""
+    return np.rint(np.asarray(x, np.float64) * 2.0 ** 133) * 2.0 ** -133
+
+
+@pytest.mark.parametrize("columns", [256, 16400])                     # rows streamed, rows resident
+def test_w4_wire_rows_every_code_under_every_scale_byte(columns):
+    """One nonzero weight in each column of y, a power of two: y names the value that a code under a byte is taken as. Byte 0 is
+    2^-127 like any other byte's power of two, and what has a block of nonzero codes under it counts."""
+    codes = np.resize(np.array([c for c in range(256) if c & 0x7F != 0x7F], np.uint8), 256)
+    place = np.arange(columns) % 256
+    w = np.zeros((columns, 128), np.uint8)
+    w[np.arange(columns), place // 2] = 2 << (4 * (place % 2))        # the code of 1
+    for exponent, some in ((125, np.arange(0, 40)), (0, np.arange(14, 247))):   # sums stay normal numbers
+        weights = weights_of(w, np.full((columns, 8), 127 + exponent, np.uint8))
+        for part in np.array_split(some, 1 + some.size // 40):
+            p, s = np.tile(codes, (part.size, 1)), np.repeat(part.astype(np.uint8)[:, None], 8, 1)
+            got = run_w4(weights, None, part.size, fp8=(p, s))
+            want = on_the_grid(R.wire_values(p, s)) * 2.0 ** exponent
+            assert np.array_equal(got, want[:, place].astype(np.float32)), part
+            assert np.array_equal(on_the_grid(R.wire_values(p, s))[part > 2], R.wire_values(p, s)[part > 2])
+
+
+@pytest.mark.parametrize("rows,n,k", [(3, 40, 160), (20, 16400, 256)])
+def test_w4_wire_rows_of_the_smallest_blocks(rows, n, k):
+    """Scale bytes 0..9 in one row, nonzero codes, under weights that make ordinary numbers of them."""
+    rng, payload, _ = w4_inputs(n, k, rows + 1)
+    w_scales = rng.integers(240, 253, (n, k // 32), dtype=np.uint8)
+    weights = weights_of(payload, w_scales)
+    p = rng.integers(1, 0x7F, (rows, k), dtype=np.uint8) | (rng.integers(0, 2, (rows, k), dtype=np.uint8) << 7)
+    s = rng.integers(0, 10, (rows, k // 32), dtype=np.uint8)
+    s[0] = 0
+    want, tol = R.w4_product(on_the_grid(R.wire_values(p, s)), R.w4_weights(payload, w_scales))
+    got = run_w4(weights, None, rows, fp8=(p, s))
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
+def test_w4_takes_the_smallest_rows_the_join_writes():
+    """A norm weight so small that the join's wire rows carry scale byte 0 over nonzero codes, read in place by a product."""
+    rows, cols, n = 5, 1024, 300
+    h, planes, _, _, _ = join_inputs(rows, cols, 1, False, "none", 21)
+    pre = np.geomspace(1e-38, 1e-34, cols).astype(np.float32)
+    out = run_join(h, planes, pre, None, None, 1.0, 1e-5, "none")
+    p, s = np.ascontiguousarray(out["payload"]), np.ascontiguousarray(out["scales"])
+    blocks = (p.reshape(rows, -1, 32) & 0x7F).any(-1)
+    assert (blocks & (s == 0)).sum() > 20 and (s > 2).sum() > 20
+    rng, payload, _ = w4_inputs(n, cols, 22)
+    w_scales = np.full((n, cols // 32), 240, np.uint8)
+    want, tol = R.w4_product(on_the_grid(R.wire_values(p, s)), R.w4_weights(payload, w_scales))
+    got = run_w4(weights_of(payload, w_scales), None, rows, fp8=(p, s))
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
 def test_w4_refuses_calls_that_do_not_fit():
     rng, payload, scales = w4_inputs(32, 64, 1)
     weights = weights_of(payload, scales)
