@@ -317,6 +317,38 @@ def test_w4_product_is_exact_on_small_integers():
     assert np.array_equal(got, (eye.astype(np.float64) @ R.w4_weights(payload, scales).T).astype(np.float32))
 
 
+# one shape or more for each form of the rule on sizes: streamed by one step and by two, resident in every number of steps and
+# waves, 16 and 32 rows a run, several runs, in phases of three and of four steps a wave, the last phase partly empty
+EXACT = [(20, 300, 1056), (16, 256, 4096), (40, 300, 12320), (16, 16500, 1024), (16, 16500, 2048), (13, 16400, 2080), (16, 9001, 4096), (9, 8300, 5152),
+         (16, 8300, 6176), (16, 17003, 8224), (5, 17003, 9248), (16, 12301, 12320), (33, 8200, 992), (64, 8200, 2048), (64, 8200, 4096), (100, 4200, 2944),
+         (64, 8300, 12320), (33, 17000, 8224)]
+
+
+@pytest.mark.parametrize("rows,n,k", EXACT)
+@pytest.mark.parametrize("form", ["bf16", "fp8"])
+def test_w4_sums_are_exact_on_small_numbers(rows, n, k, form):
+    """Weights are multiples of 1/4 up to 12 and values multiples of 1/2 up to 8, so that a sum over k is a multiple of 1/8 of at most 96 k, which
+    is under 2^24 of them for k up to 21845: any order of FP32 additions is exact, and sums held in anything less are not."""
+    assert 96 * k * 8 < 1 << 24
+    period = min(n, 1021)                                             # weight rows repeat after a prime number of them: no whole tiles
+    rng, payload, _ = w4_inputs(period, k, rows + n + k)
+    scales = rng.integers(126, 129, (period, k // 32), dtype=np.uint8)
+    again = np.arange(n) % period
+    weights = weights_of(payload[again], scales[again])
+    integers = rng.integers(-4, 5, (rows, k))
+    s = rng.integers(126, 129, (rows, k // 32), dtype=np.uint8)
+    value = (integers * np.exp2(np.repeat(s, 32, 1).astype(np.float64) - 127)).astype(np.float32)
+    if form == "bf16":
+        got = run_w4(weights, R.bf16(value)[0], rows)
+    else:
+        code = np.array([0, 0x38, 0x40, 0x44, 0x48], np.uint8)         # E4M3 of 0..4
+        p = code[np.abs(integers)] | np.where(integers < 0, 0x80, 0).astype(np.uint8)
+        assert np.array_equal(R.wire_values(p, s), value)
+        got = run_w4(weights, None, rows, fp8=(p, s))
+    want = value.astype(np.float64) @ R.w4_weights(payload, scales).T
+    assert np.array_equal(got, want[:, again]), np.argwhere(got != want[:, again])[:4]
+
+
 def test_w4_scale_bytes_every_one_accepted_or_refused():
     """Scale bytes 2..252 over nonzero codes are exact single products, groups of zeros carry any byte, and any other byte over a
     nonzero code is refused (code 3)."""
