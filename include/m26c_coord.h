@@ -84,11 +84,12 @@ int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_
  * A logit of -infinity is a masked token: probability 0, log probability -infinity, never an alternative; where fewer than
  * `top` are left, the id is -1 and the log probability -infinity. A row with nothing left gives -infinity, entropy 0
  * and no alternatives. NaN or +infinity in a row makes its log probabilities and entropy NaN (ids stay ordered; a
- * NaN is never an alternative). given / given_logprob may be null when n_given is 0, the top arrays when top is 0, entropy
- * always. 0 <= top <= min(32, vocab), vocab and n_given <= 2^30. `workspace`: at least m26c_token_logprobs_workspace(rows, vocab,
- * top) bytes, 16-byte aligned, its content irrelevant before and after; may be null when that is 0. Fewer rows may need
- * more; 8192 * (16 + 8 * top) bytes do for any call. Calls that may overlap need workspaces of their own. A row's values do
- * not depend on the other rows; which sums are formed first, and with that the last bits, depends on rows and vocab. */
+ * NaN is never an alternative). Log probabilities are never above 0 and entropies never below. given / given_logprob may be
+ * null when n_given is 0, the top arrays when top is 0, entropy always. 0 <= top <= min(32, vocab), vocab and n_given <= 2^30.
+ * `workspace`: at least m26c_token_logprobs_workspace(rows, vocab, top) bytes, 16-byte aligned, its content irrelevant before
+ * and after; may be null when that is 0. Fewer rows may need more; 8192 * (16 + 8 * top) bytes do for any call. Calls that may
+ * overlap need workspaces of their own. A row's values do not depend on the other rows; which sums are formed first, and with
+ * that the last bits, depends on rows and vocab. */
 size_t m26c_token_logprobs_workspace(int rows, int vocab, int top);
 int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int vocab, float scale, const int* given, int n_given,
                         float* given_logprob, float* entropy, int top, int* top_ids, float* top_logprob, void* workspace,

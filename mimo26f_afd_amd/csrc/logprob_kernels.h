@@ -387,9 +387,12 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
     constexpr float kLn2 = 0.69314718055994531f;
     const bool empty = sum.m == -INFINITY && sum.z == 0.0f;
     // Z is relative to 2^r, r = m c rounded: what r is short of m c is exactly a fused product
-    const float ln_z = kLn2 * (SoftmaxSums::far(sum.m, c) || sum.m == -INFINITY ? log_z : log_z - __builtin_fmaf(sum.m, c, -(sum.m * c)));
+    // Z relative to 2^(m c) is one at least and the entropy zero at least: what the roundings leave below counts as that (one token left)
+    // and a NaN goes through.
+    auto not_below_zero = [](float v) { return v <= 0.0f ? 0.0f : v; };
+    const float ln_z = kLn2 * not_below_zero(SoftmaxSums::far(sum.m, c) || sum.m == -INFINITY ? log_z : log_z - __builtin_fmaf(sum.m, c, -(sum.m * c)));
     auto logprob = [&](float v) { return (v - sum.m) * a.scale - ln_z; };
-    if (tid == 0 && a.entropy) a.entropy[row] = empty ? 0.0f : kLn2 * (log_z - sum.s / sum.z);
+    if (tid == 0 && a.entropy) a.entropy[row] = empty ? 0.0f : kLn2 * not_below_zero(log_z - sum.s / sum.z);
     for (int i = tid; i < a.n_given; i += THREADS) {
         if (i >= THREADS) given = given_logit<BF16>(a, row, i);
         a.given_logprob[row * a.n_given + i] = !given.there ? __builtin_nanf("") : empty ? -INFINITY : logprob(given.v);

@@ -685,6 +685,26 @@ def test_logprobs_of_hard_rows_among_many(half, vocab, copies, top):
         assert (bits == bits[:1]).all()
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(2000, 700), (300, 5003), (700, 5003), (30, 50003), (200, 50003)])
+def test_logprobs_are_never_above_zero_and_entropies_never_below(rows, vocab, half):
+    """Constrained decoding: one allowed token, or one far ahead of a few others, at any logit, with every one of them given."""
+    rng = np.random.default_rng(rows + vocab)
+    x = np.full((rows, vocab), -np.inf, np.float32)
+    at = rng.integers(0, vocab, (rows, 3))
+    x[np.arange(rows), at[:, 0]] = rng.standard_normal(rows) * np.exp2(rng.integers(-3, 12, rows))
+    some = np.arange(rows) % 4 == 0
+    for i in (1, 2):
+        x[some, at[some, i]] = x[some, at[some, 0]] - rng.integers(15, 40, some.sum())
+    x = R.bf16(x)[1] if half else x
+    for scale in (1.0, 0.7):
+        got = run_logprobs(x, at, 2, scale, half)
+        check_logprobs(got, x, at, 2, scale)
+        given, entropy, _, top = got
+        assert (given <= 0).all() and (top <= 0).all() and (entropy >= 0).all(), (given.max(), top.max(), entropy.min())
+        assert not np.signbit(entropy).any()
+
+
 def test_logprobs_signalling_nans_do_not_hide_values():
     x = np.random.default_rng(3).standard_normal((4, 3000)).astype(np.float32)
     raw = x.view(np.uint32)
