@@ -391,7 +391,8 @@ __device__ __forceinline__ void write_row(const LogprobArgs& a, long row, const 
     // and a NaN goes through.
     auto not_below_zero = [](float v) { return v <= 0.0f ? 0.0f : v; };
     const float ln_z = kLn2 * not_below_zero(SoftmaxSums::far(sum.m, c) || sum.m == -INFINITY ? log_z : log_z - __builtin_fmaf(sum.m, c, -(sum.m * c)));
-    auto logprob = [&](float v) { return (v - sum.m) * a.scale - ln_z; };
+    // halves, so that the difference of two numbers is one
+    auto logprob = [&](float v) { return (0.5f * v - 0.5f * sum.m) * (2.0f * a.scale) - ln_z; };
     if (tid == 0 && a.entropy) a.entropy[row] = empty ? 0.0f : kLn2 * not_below_zero(log_z - sum.s / sum.z);
     for (int i = tid; i < a.n_given; i += THREADS) {
         if (i >= THREADS) given = given_logit<BF16>(a, row, i);

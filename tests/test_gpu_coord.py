@@ -705,6 +705,20 @@ def test_logprobs_are_never_above_zero_and_entropies_never_below(rows, vocab, ha
         assert not np.signbit(entropy).any()
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("rows,vocab", [(3, 700), (40, 5003), (700, 5003), (3, 50003), (200, 50003)])
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** -122, 2.0 ** -135])
+def test_logprobs_of_logits_whose_differences_pass_fp32(rows, vocab, half, scale):
+    """Logits over FP32's whole range, brought to ordinary sizes by the scale: a difference of two may be past the range."""
+    rng = np.random.default_rng(rows + vocab)
+    x = rng.uniform(-3.38e38, 3.38e38, (rows, vocab)).astype(np.float32)
+    x[:, 5], x[:, vocab // 2] = 3.38e38, -3.38e38
+    x[rng.random((rows, vocab)) < 0.1] = -np.inf
+    x = R.bf16(x)[1] if half else x
+    given = np.stack([[5, vocab // 2, 0]] * rows)
+    check_logprobs(run_logprobs(x, given, 8, scale, half), x, given, 8, scale)
+
+
 def test_logprobs_signalling_nans_do_not_hide_values():
     x = np.random.default_rng(3).standard_normal((4, 3000)).astype(np.float32)
     raw = x.view(np.uint32)
