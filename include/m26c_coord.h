@@ -58,7 +58,8 @@ int m26c_block_join(const m26c_join* plan, long rows, const float* h, const uint
  * k a multiple of 32, n and k up to 2^24, and so are the pitches of x and y. m26c_w4_new lays them out once in the order the
  * matrix pipe reads, on the current device, and waits for that; the sources may be freed afterwards. Scale bytes have to lie in [2, 252] wherever a group holds a
  * nonzero code (the format's range in which every product is a normal number); a group of zeros may carry any byte.
- * Returns 1 for a bad argument, 2 for a failed allocation or launch, 3 for a scale byte out of that range. */
+ * Returns 1 for a bad argument or a stream that is being captured, 2 for a failed allocation or launch, 3 for a scale byte out
+ * of that range. */
 typedef struct m26c_w4 m26c_w4;
 int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, void* stream, m26c_w4** out, char* err, size_t errlen);
 void m26c_w4_free(m26c_w4* w);

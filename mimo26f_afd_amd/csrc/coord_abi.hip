@@ -249,6 +249,10 @@ int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, v
     *out = nullptr;
     if (!payload || !scales || n <= 0 || k <= 0 || k % 32 || n > kPitchMost || k > kPitchMost) return fail(err, errlen, 1, "w4 weights: bad pointers or sizes");
     if (!on(payload, 16)) return fail(err, errlen, 1, "w4 weights: the payload has to be 16-byte aligned");
+    hipStream_t st = hipStream_t(stream);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &capture) != hipSuccess) (void)hipGetLastError();  // no device: the allocation below says so
+    if (capture != hipStreamCaptureStatusNone) return fail(err, errlen, 1, "w4 weights: the stream is being captured");
     m26c_w4* w = new (std::nothrow) m26c_w4{};
     if (!w) return fail(err, errlen, 2, "w4 weights: out of host memory");
     w->lay = W4Layout{n, k, int((n + 15) / 16), int((k + 127) / 128), int((k + 511) / 512)};
@@ -261,7 +265,6 @@ int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, v
         return fail(err, errlen, 2, "w4 weights: device allocation failed");
     }
     fault = w->scales + scale_bytes / 4;  // one word behind the scales
-    hipStream_t st = hipStream_t(stream);
     uint32_t seen = 0;
     const long cells = long(w->lay.tiles) * w->lay.quads * 256;
     const long blocks = (cells + 255) / 256;
@@ -273,6 +276,7 @@ int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, v
     if (e == hipSuccess) e = hipMemcpyAsync(&seen, fault, 4, hipMemcpyDeviceToHost, st);
     if (e == hipSuccess) e = hipStreamSynchronize(st);
     if (e != hipSuccess || seen) {
+        (void)hipGetLastError();  // reported here, not by the next launch
         release(w);
         return e != hipSuccess ? fail(err, errlen, 2, hipGetErrorString(e))
                                : fail(err, errlen, 3, "w4 weights: a scale byte outside 2..252 over a nonzero code");

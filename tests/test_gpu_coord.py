@@ -919,3 +919,31 @@ def test_captured_step_replays_on_new_inputs_beside_eager_calls():
     hip("hipGraphDestroy", graph)
     hip("hipStreamDestroy", side)
     hip("hipStreamDestroy", other)
+
+
+def test_weights_are_not_laid_out_within_a_capture_and_leave_it_whole():
+    """Laying weights out waits for the stream, which a capture does not allow: refused before anything is done, so that the graph
+    goes on and no later call reports the failure."""
+    hip = Hip()
+    rng, payload, scales = w4_inputs(40, 128, 3)
+    weights, p, s = weights_of(payload, scales), dev(payload), dev(scales)
+    bits, value = R.bf16(rng.standard_normal((2, 128)).astype(np.float32))
+    x, y = dev(bits), room(2 * 40 * 4)
+    side, graph, runnable = hip.stream(), C.c_void_p(), C.c_void_p()
+    hip("hipStreamBeginCapture", side, C.c_int(2))                    # relaxed
+    with pytest.raises(coord.CoordError) as e:
+        coord.Weights4(p.ptr, s.ptr, 40, 128, stream=side.value)
+    assert e.value.code == 1 and "captured" in str(e.value)
+    weights.matvec(x.ptr, 2, y.ptr, stream=side.value)
+    hip("hipStreamEndCapture", side, C.byref(graph))
+    hip("hipPeekAtLastError")
+    hip("hipGraphInstantiate", C.byref(runnable), graph, None, None, C.c_size_t(0))
+    want, tol = R.w4_product(value, R.w4_weights(payload, scales))
+    for _ in range(3):
+        put(y.ptr, np.full(2 * 40, 7.0, np.float32))
+        hip("hipGraphLaunch", runnable, side)
+        hip("hipStreamSynchronize", side)
+        assert np.all(np.abs(y.to_host(np.float32).reshape(2, 40) - want) <= tol)
+    hip("hipGraphExecDestroy", runnable)
+    hip("hipGraphDestroy", graph)
+    hip("hipStreamDestroy", side)
