@@ -24,6 +24,13 @@ def _ck(code: int, what: str) -> None:
         raise CoordError(code, what)
 
 
+def _int(v: int, what: str) -> int:
+    """`v`, refused where C's int would hold another number."""
+    if not -0x80000000 <= v <= 0x7FFFFFFF:
+        raise CoordError(1, what)
+    return v
+
+
 class _JoinPlan(C.Structure):
     _fields_ = [("cols", C.c_int), ("planes", C.c_int), ("plane_pitch", C.c_long), ("h_pitch", C.c_long), ("norm_pitch", C.c_long),
                 ("pre_weight", C.c_void_p), ("post_weight", C.c_void_p), ("gate_cols", C.c_int), ("gate_pitch", C.c_long),
@@ -38,6 +45,8 @@ class Join:
     def __init__(self, cols: int, pre_weight: int | None, post_weight: int | None = None, planes: int = 1, gate_cols: int = 0,
                  gate_pitch: int = 0, scale: float = 1.0, eps: float = 1e-6, plane_pitch: int = 0, h_pitch: int = 0,
                  norm_pitch: int = 0, payload_pitch: int = 0, scales_pitch: int = 0):
+        for v in (cols, planes, gate_cols):
+            _int(v, "block join")
         self._plan = _JoinPlan(cols, planes, plane_pitch or cols, h_pitch or cols, norm_pitch or cols, pre_weight, post_weight, gate_cols,
                                gate_pitch, scale, eps, payload_pitch or cols, scales_pitch or cols // 32)
         self._ref = C.byref(self._plan)
@@ -70,13 +79,13 @@ class Weights4:
 
     def matvec(self, x: int, rows: int, y: int, y_bf16: bool = False, x_pitch: int = 0, y_pitch: int = 0, stream: int | None = None) -> None:
         """y = x W^T for `rows` BF16 rows; FP32 out, or BF16."""
-        _ck(self._bf16(self._h, x, x_pitch or self.k, rows, y, y_bf16, y_pitch or self.n, stream), "w4 product")
+        _ck(self._bf16(self._h, x, x_pitch or self.k, _int(rows, "w4 product"), y, y_bf16, y_pitch or self.n, stream), "w4 product")
 
     def matvec_fp8(self, payload: int, scales: int, rows: int, y: int, y_bf16: bool = False, payload_pitch: int = 0,
                    scales_pitch: int = 0, y_pitch: int = 0, stream: int | None = None) -> None:
         """The same for wire rows (E4M3 codes, one UE8M0 byte per 32 values)."""
-        _ck(self._fp8(self._h, payload, payload_pitch or self.k, scales, scales_pitch or self.k // 32, rows, y, y_bf16, y_pitch or self.n,
-                      stream), "w4 product of wire rows")
+        _ck(self._fp8(self._h, payload, payload_pitch or self.k, scales, scales_pitch or self.k // 32, _int(rows, "w4 product of wire rows"), y,
+                      y_bf16, y_pitch or self.n, stream), "w4 product of wire rows")
 
     def close(self) -> None:
         if getattr(self, "_h", None) and self._h.value and load is not None:  # load is gone at interpreter exit
@@ -88,6 +97,8 @@ class Weights4:
 
 def token_logprobs_workspace(rows: int, vocab: int, top: int) -> int:
     """Bytes of device memory token_logprobs needs for these sizes (0: none)."""
+    if max(rows, vocab, top) > 0x7FFFFFFF or min(rows, vocab, top) < 0:
+        return 0
     return int(load().m26c_token_logprobs_workspace(rows, vocab, top))
 
 
@@ -96,5 +107,7 @@ def token_logprobs(logits: int, bf16: bool, rows: int, vocab: int, pitch: int, g
                    workspace_bytes: int, scale: float = 1.0, stream: int | None = None) -> None:
     """Log softmax of scale * logits at `given` [rows][n_given] (int32; an id outside the vocabulary gives NaN), its entropy per
     row and its `top` largest values with their ids (-1 where masked logits leave fewer)."""
+    for v in (rows, vocab, n_given, top):
+        _int(v, "token log probabilities")
     _ck(load().m26c_token_logprobs(logits, bf16, pitch, rows, vocab, scale, given, n_given, given_logprob, entropy, top, top_ids,
                                    top_logprob, workspace, workspace_bytes, stream), "token log probabilities")

@@ -81,6 +81,23 @@ def test_logprobs_refuse(change):
     refused(logprob_call, **change)
 
 
+@pytest.mark.parametrize("past", [1 << 32, -(1 << 32)])
+def test_sizes_past_an_int_are_refused_not_wrapped(past):
+    """A size that C's int does not hold would come through as another one, and a part of the rows be answered."""
+    for change in (dict(rows=past + 2), dict(vocab=past + 100, pitch=1 << 33), dict(n_given=past + 1), dict(top=past + 3)):
+        refused(logprob_call, **change)
+    assert coord.token_logprobs_workspace(past + 1, 131072, 5) == 0 and coord.token_logprobs_workspace(1, past + 131072, 5) == 0
+    for change in (dict(cols=past + 64, plane_pitch=1 << 33, h_pitch=1 << 33, norm_pitch=1 << 33), dict(planes=past + 1), dict(gate_cols=past)):
+        refused(join_call, dict(GOOD, **change), norm=P, gate=P)
+    weights = coord.Weights4.__new__(coord.Weights4)                  # no handle: nothing would run
+    weights._h, weights.n, weights.k = C.c_void_p(), 16, 64
+    ran = []
+    weights._bf16 = weights._fp8 = lambda *a: ran.append(a) or 0
+    refused(weights.matvec, P, past + 1, P)
+    refused(weights.matvec_fp8, P, P, past + 1, P)
+    assert not ran
+
+
 def test_logprobs_of_no_rows_and_their_workspace():
     logprob_call(rows=0)
     assert coord.token_logprobs_workspace(0, 1000, 5) == 0 and coord.token_logprobs_workspace(-1, 1000, 5) == 0
