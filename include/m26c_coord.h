@@ -54,10 +54,11 @@ int m26c_block_join(const m26c_join* plan, long rows, const float* h, const uint
 
 /* ---- products with MXFP4 weights -----------------------------------------------------------------------
  * y[r][j] = sum over k of x[r][k] * e2m1(code[j][k]) * 2^(scale[j][k / 32] - 127)
- * Weights in the checkpoint's own form: [n][k / 2] payload bytes, low nibble = even k, [n][k / 32] scale bytes;
- * k a multiple of 32, n and k up to 2^24, and so are the pitches of x and y. m26c_w4_new lays them out once in the order the
- * matrix pipe reads, on the current device, and waits for that; the sources may be freed afterwards. Scale bytes have to lie in [2, 252] wherever a group holds a
- * nonzero code (the format's range in which every product is a normal number); a group of zeros may carry any byte.
+ * Weights in the form the experts' MXFP4 has in a checkpoint: [n][k / 2] payload bytes, low nibble = even k, 16-byte aligned,
+ * [n][k / 32] scale bytes at any alignment; k a multiple of 32, n and k up to 2^24, and so are the pitches of x and y.
+ * m26c_w4_new lays them out once in the order the matrix pipe reads, on the current device, and waits for that; the sources may
+ * be freed afterwards. Scale bytes have to lie in [2, 252] wherever a group holds a nonzero code (the format's range in which
+ * every weight is a normal number); a group of zeros may carry any byte.
  * Returns 1 for a bad argument or a stream that is being captured, 2 for a failed allocation or launch, 3 for a scale byte out
  * of that range. */
 typedef struct m26c_w4 m26c_w4;

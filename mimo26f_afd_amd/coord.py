@@ -65,8 +65,8 @@ class Join:
 
 
 class Weights4:
-    """[n][k] MXFP4 weights (payload [n][k / 2], low nibble = even k; one E8M0 byte per 32 k), laid out once on the current
-    device; the sources may be freed afterwards."""
+    """[n][k] MXFP4 weights (payload [n][k / 2], low nibble = even k, 16-byte aligned; one E8M0 byte per 32 k, at any alignment), laid
+    out once on the current device; the sources may be freed afterwards."""
 
     def __init__(self, payload: int, scales: int, n: int, k: int, stream: int | None = None):
         self._h = C.c_void_p()
