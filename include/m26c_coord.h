@@ -30,7 +30,9 @@ extern "C" {
  * the rule of m26c_quantize_hidden, taken from the FP32 n. Sums are FP32 (a row whose sum of squares passes FP32's range is
  * normed to zero). A NaN or an infinity of a row stays in its row.
  * The plan holds what a program keeps from call to call. Pitches count elements (bytes for payload and scales); rows of
- * `cols` values, 1 <= cols <= 16384, a multiple of 32 for wire rows. Any alignment of the element type is accepted. */
+ * `cols` values, 1 <= cols <= 16384, a multiple of 32 for wire rows. Any alignment of the element type is accepted. A row's values
+ * do not depend on the other rows; the order of its sums, and with that their last bits, depends on cols and, between
+ * 2048 and 8192 of them, on whether the call has 512 rows or more. */
 typedef struct m26c_join {
     int cols;
     int planes;               /* 1..4 */
@@ -66,8 +68,9 @@ int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, v
 void m26c_w4_free(m26c_w4* w);
 
 /* x: BF16 rows at x_pitch elements, 16-byte aligned and the pitch a multiple of 8. y: FP32, or BF16 (nearest even) when
- * y_bf16 is not 0, rows at y_pitch elements. Sums are FP32. Made for up to 64 rows; any number is
- * taken, 16 or 32 at a time. The current device has to be the one the weights are on. */
+ * y_bf16 is not 0, rows at y_pitch elements. Sums are FP32; their order, and with that the last bits, depends on rows, n and k. Made
+ * for up to 64 rows; any number is taken, 16 or 32 at a time, which widens the weights again for each (4096 x 4096: 512 rows 28 us,
+ * 2048 rows 179). The current device has to be the one the weights are on. */
 int m26c_w4_matvec(const m26c_w4* w, const uint16_t* x, long x_pitch, int rows, void* y, int y_bf16, long y_pitch, void* stream);
 
 /* The same on wire rows: E4M3 codes and one UE8M0 byte per 32 values, at their own pitches in bytes (request-frame rows are
@@ -91,7 +94,7 @@ int m26c_w4_matvec_fp8(const m26c_w4* w, const uint8_t* payload, size_t payload_
  * `workspace`: at least m26c_token_logprobs_workspace(rows, vocab, top) bytes, 16-byte aligned, its content irrelevant before
  * and after; may be null when that is 0. Fewer rows may need more; 8192 * (16 + 8 * top) bytes do for any call. Calls that may
  * overlap need workspaces of their own. A row's values do not depend on the other rows; which sums are formed first, and with
- * that the last bits, depends on rows and vocab. */
+ * that the last bits, depends on rows and vocab and, in long rows, on a row's address modulo 16. */
 size_t m26c_token_logprobs_workspace(int rows, int vocab, int top);
 int m26c_token_logprobs(const void* logits, int bf16, long pitch, int rows, int vocab, float scale, const int* given, int n_given,
                         float* given_logprob, float* entropy, int top, int* top_ids, float* top_logprob, void* workspace,

@@ -3,10 +3,10 @@
 //   Z = sum exp(t - m),  S = sum exp(t - m) (t - m)
 //   log p(j) = t_j - m - ln Z,   entropy = ln Z - S / Z,   the largest logits in descending order, equal ones by the lower id
 //
-// The logits are read once, which is the bound of large calls: everything else is a few values per row. About nine vector
-// instructions a value (one of them an exponential) are four fifths of what the chip does in the time HBM needs for a BF16
-// value, so the selection may add next to nothing to the common path: 2048 rows x 131072 BF16, top 5, 537 MB in 96 us (5.6
-// TB/s, 84 % of a streaming read). Small calls are chains of dependent steps: 1 row x 131072 9.8 us, two launches 4 of them.
+// The logits are read once, which is the bound of large calls: everything else is a few values per row. The vector instructions
+// (10.9 a BF16 value counted, one of them an exponential) keep their pipe busy 78 % of the counted cycles of such a call,
+// so the selection may add next to nothing to the common path: 2048 rows x 131072 BF16, top 5, 537 MB in 98 us (5.5
+// TB/s, 82 % of a streaming read). Small calls are chains of dependent steps: 1 row x 131072 9.8 us, two launches 4 of them.
 //
 // Two forms. Many long rows are walked, as follows; few rows or short ones are held in registers (short_part below).
 //
