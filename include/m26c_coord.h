@@ -6,7 +6,8 @@
  * current device; `stream` is a hipStream_t (or null) of that device. The calls only launch (m26c_w4_new apart) and may be
  * captured into a graph. Return value: 0 on success, 1 for a bad argument (nothing is launched then), otherwise the
  * hipError_t of the failed launch. Nothing is kept between calls but what a caller passes in, so calls on different
- * streams may run at once as long as they write different memory.
+ * streams may run at once as long as they write different memory. Outputs may not overlap inputs but where that is said. A
+ * graph reads what its calls were given at each replay, a handle's weights among them: they have to live as long as it.
  *
  * The reference does these steps in separate kernels of its coordinator (crates/mimo26-coordinator/kernels/glue.cu, lm8.cu, sample.cu);
  * the entries here have no counterpart of the same form.
@@ -28,7 +29,7 @@ extern "C" {
  *   n  = h' * pre_weight / sqrt(mean(h'^2) + eps)
  * Outputs: h' (FP32), and n as BF16 (nearest even) and / or as wire rows: E4M3 codes with one UE8M0 byte per 32 values by
  * the rule of m26c_quantize_hidden, taken from the FP32 n. Sums are FP32 (a row whose sum of squares passes FP32's range is
- * normed to zero). A NaN or an infinity of a row stays in its row.
+ * normed to zero; squares under 2^-126 lose bits, which shows beside an eps as small only). A NaN or an infinity of a row stays in its row.
  * The plan holds what a program keeps from call to call. Pitches count elements (bytes for payload and scales); rows of
  * `cols` values, 1 <= cols <= 16384, a multiple of 32 for wire rows. Any alignment of the element type is accepted. A row's values
  * do not depend on the other rows; the order of its sums, and with that their last bits, depends on cols and, between

@@ -24,7 +24,8 @@ void launch_join(const JoinArgs& a, hipStream_t st) {
 }
 
 // ---- log probabilities
-// How a call is cut, by rows and vocabulary alone (us a pass; walking / short parts):
+// How a call is cut, by rows and vocabulary alone (us a pass inside a captured graph on inputs in turn, as everywhere in this file; where a
+// rule turns, both forms were timed at sizes on either side of it; walking / short parts):
 //  * up to two waves' registers hold a row: a workgroup per row, short parts (16384 x 1000 BF16, top 5: 39 / 26)
 //  * up to eight, as long as the chip holds all rows at once (512 x 8000, top 5: 11.8 / 9.6; 2048 x 8000 18.1 / 30.2 the other way)
 //  * few rows: over several workgroups in short parts of two chunks, of four where 128 parts would not reach (1 row x 131072
