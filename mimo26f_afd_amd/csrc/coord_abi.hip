@@ -252,7 +252,7 @@ int m26c_w4_new(const uint8_t* payload, const uint8_t* scales, long n, long k, v
     if (!on(payload, 16)) return fail(err, errlen, 1, "w4 weights: the payload has to be 16-byte aligned");
     hipStream_t st = hipStream_t(stream);
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(st, &capture) != hipSuccess) (void)hipGetLastError();  // no device: the allocation below says so
+    if (hipStreamIsCapturing(st, &capture) != hipSuccess) (void)hipGetLastError();  // no device, say: what follows reports it
     if (capture != hipStreamCaptureStatusNone) return fail(err, errlen, 1, "w4 weights: the stream is being captured");
     m26c_w4* w = new (std::nothrow) m26c_w4{};
     if (!w) return fail(err, errlen, 2, "w4 weights: out of host memory");
